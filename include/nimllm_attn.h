@@ -185,6 +185,8 @@ int nimllm_rope_append_paged(void *q, int n_head, void *k_new, const void *v_new
  *                            machines without a GPU) -- k(), v() and table() then return NULL
  *   reserve(seq, rows_total) pages for rows 0 .. rows_total-1 of sequence slot `seq`; never shrinks
  *   release(seq)             all pages of the slot back to the free list
+ *   shrink(seq, rows_total)  the pages past rows_total rows back to the free list (after an eviction, or
+ *                            drafts that were not accepted); more rows than it holds change nothing
  *   sync(stream)             uploads the table rows changed since the last sync, on `stream`,
  *                            before the launches that read them
  *   table(first_seq)         device int32 [max_seqs - first_seq][max_pages]: the page_table
@@ -198,6 +200,7 @@ nimllm_kvpool *nimllm_kvpool_create(int n_layer, int n_pages, int page_rows, int
 void nimllm_kvpool_destroy(nimllm_kvpool *pool);
 int nimllm_kvpool_reserve(nimllm_kvpool *pool, int seq, int rows_total);
 int nimllm_kvpool_release(nimllm_kvpool *pool, int seq);
+int nimllm_kvpool_shrink(nimllm_kvpool *pool, int seq, int rows_total);
 int nimllm_kvpool_sync(nimllm_kvpool *pool, void *stream);
 int nimllm_kvpool_free_pages(const nimllm_kvpool *pool);
 int nimllm_kvpool_seq_pages(const nimllm_kvpool *pool, int seq);
@@ -206,6 +209,134 @@ const int32_t *nimllm_kvpool_table_host(const nimllm_kvpool *pool);
 const int32_t *nimllm_kvpool_table(const nimllm_kvpool *pool, int first_seq);
 void *nimllm_kvpool_k(const nimllm_kvpool *pool, int layer);
 void *nimllm_kvpool_v(const nimllm_kvpool *pool, int layer);
+
+/* ---- a cache whose rows are not its positions: drafted trees and evicted caches ------------------
+ * No counterpart in the reference, where row == position everywhere (src/model.nim:788-840).  Two
+ * ways in which that ends: several drafted continuations of a sequence sit in the cache at once and
+ * share positions, and rows that attention hardly uses are dropped to make room.  The calls of a step:
+ *
+ *   nimllm_rope_append_at       drafted tokens: q and k rotated at their depth, rows appended in order
+ *   nimllm_attn_decode_tree     their attention over the committed rows and over each other
+ *   nimllm_kv_accept            the rows of the accepted path moved down behind the committed ones
+ *   nimllm_attn_decode_scored   a decode step that adds up every cached row's attention weight
+ *   nimllm_kv_evict             the rows with the largest sums kept, the others given up
+ *
+ * Every one takes the contiguous layout (kv_off / seq_stride / head_stride / max_seq rows per block)
+ * or, with _paged, pages (page_rows a power of two >= 32; n_pages the size of the pool).  Rows at or
+ * past max_seq (max_pages * page_rows) and rows whose table entry is outside [0, n_pages) do not
+ * exist: they are not read, stored, attended or moved.  Cache pointers and strides are multiples of
+ * 16 bytes.  Lengths in device arrays are clamped to what the host arguments allow.  All calls can be
+ * captured in a CUDA graph; calls that may overlap on the GPU need workspaces of their own. */
+#define NIMLLM_ROPE_HALF 0        /* pairs (f, f + rot_dim/2), as the reference rotates */
+#define NIMLLM_ROPE_INTERLEAVED 1 /* pairs (2f, 2f + 1) */
+#define NIMLLM_ROPE_SCALE_NONE 0
+#define NIMLLM_ROPE_SCALE_LINEAR 1 /* every frequency divided by factor */
+#define NIMLLM_ROPE_SCALE_BASE 2   /* base * factor^(rot_dim / (rot_dim - 2)): the slowest frequency divided by factor */
+#define NIMLLM_ROPE_SCALE_RAMP 3   /* by the turns t a frequency makes over orig_len positions: t >= high kept, t <= low
+                                      divided by factor, linear in t between */
+
+/* cos / sin tables [max_pos, rot_dim/2] on the HOST for positions past the trained length.  Angles are
+ * 64-bit up to the rounding of the table.  gain multiplies both tables (1: none); low, high and
+ * orig_len are read for the ramp only. */
+int nimllm_rope_tables_scaled_host(float *cos_tab, float *sin_tab, int max_pos, int rot_dim, double base, int kind,
+                                   double factor, double low, double high, int orig_len, double gain);
+
+/* Rotation and append with a position and a row of their own per token.
+ *   q, q_out    [batch, n, n_head*head_dim] act_dtype, q_out may be q (both NULL: none)
+ *   k_new       [batch, n, n_kv_head*head_dim]; k_out optional rotated copy (may be k_new)
+ *   v_new       as k_new, copied raw into the cache
+ *   rope tables [table_rows, rot_dim/2]; the first rot_dim columns of a head rotate (a multiple of 8),
+ *               the others pass; both tables NULL: nothing rotates
+ *   pos         device int32 [batch, n], or NULL: the token's row.  A token with a negative position or
+ *               one past the table is padding: nothing of it is read or written
+ *   row0        device int32 [batch], cache row of each sequence's token 0, or NULL: first_row
+ *   caches NULL: rotate only
+ * nimllm_rope_at_bwd is the gradient of the rotation: dq = R^T dq_rot, dk = R^T dk_rot (in place or
+ * not; zero for padding; pos NULL: position pos0 + t). */
+int nimllm_rope_append_at(const void *q, void *q_out, int n_head, const void *k_new, void *k_out, const void *v_new,
+                          int act_dtype, const float *rope_cos, const float *rope_sin, int rot_dim, int layout,
+                          int table_rows, const int32_t *pos, const int32_t *row0, int first_row, void *k_cache,
+                          void *v_cache, int cache_dtype, const int64_t *kv_off, int64_t seq_stride, int64_t head_stride,
+                          int max_seq, int batch, int n, int n_kv_head, int head_dim, void *stream);
+int nimllm_rope_append_at_paged(const void *q, void *q_out, int n_head, const void *k_new, void *k_out,
+                                const void *v_new, int act_dtype, const float *rope_cos, const float *rope_sin,
+                                int rot_dim, int layout, int table_rows, const int32_t *pos, const int32_t *row0,
+                                int first_row, void *k_pages, void *v_pages, int cache_dtype, const int32_t *page_table,
+                                int max_pages, int page_rows, int n_pages, int batch, int n, int n_kv_head, int head_dim,
+                                void *stream);
+int nimllm_rope_at_bwd(const void *dq_rot, void *dq, int n_head, const void *dk_rot, void *dk, int dtype,
+                       const float *rope_cos, const float *rope_sin, int rot_dim, int layout, int table_rows,
+                       const int32_t *pos, int pos0, int batch, int n, int n_kv_head, int head_dim, void *stream);
+
+/* Attention of n (<= 256) drafted tokens per sequence.  Sequence b has seq_len[b] committed rows, which all
+ * of its tokens attend; its draft j is row seq_len[b] + j, already appended.
+ *   q          [batch, n, n_head*head_dim] q_dtype, rotated;  out the same shape, out_dtype
+ *   seq_len    device int32 [batch] in 0 .. max_len, or NULL: max_len for all
+ *   n_new      device int32 [batch], drafts of each sequence, or NULL: n.  Rows of out past them are left as they were
+ *   tree_mask  device uint64 [batch, n, (n + 63) / 64]: bit j of token i's words, it attends draft j (its
+ *              ancestors and itself); NULL: a chain, drafts 0 .. i.  A token without any row to attend gets zeros
+ *   partials_out  optional fp32 [batch*n*n_head, head_dim + 4] records as in nimllm_attn_decode (out may be NULL then)
+ *   head_dim   64 or 128.  The products are those of 32-bit arithmetic for either cache type; every row of V up to the last
+ *              draft must be finite even where a mask hides it (a hidden row of K may hold anything)
+ *   workspace  256-byte aligned, nimllm_attn_decode_tree_workspace_bytes(...) bytes */
+size_t nimllm_attn_decode_tree_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, int max_len,
+                                               int cache_dtype);
+int nimllm_attn_decode_tree(const void *q, int q_dtype, const void *k_cache, const void *v_cache, int cache_dtype,
+                            const int64_t *kv_off, int64_t seq_stride, int64_t head_stride, int max_seq,
+                            const int32_t *seq_len, int max_len, const int32_t *n_new, const uint64_t *tree_mask, void *out,
+                            int out_dtype, float *partials_out, int batch, int n, int n_head, int n_kv_head, int head_dim,
+                            float scale, void *workspace, size_t workspace_bytes, void *stream);
+int nimllm_attn_decode_tree_paged(const void *q, int q_dtype, const void *k_pages, const void *v_pages, int cache_dtype,
+                                  const int32_t *page_table, int max_pages, int page_rows, int n_pages,
+                                  const int32_t *seq_len, int max_len, const int32_t *n_new, const uint64_t *tree_mask,
+                                  void *out, int out_dtype, float *partials_out, int batch, int n, int n_head, int n_kv_head,
+                                  int head_dim, float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* After the drafts were checked: row seq_len[b] + i of K and V becomes the former row seq_len[b] + path[b][i], for
+ * i < n_path[b], in n_layer layers that lie layer_stride elements apart, and new_len[b] = seq_len[b] + the number of
+ * accepted rows (new_len may be seq_len).  A path lists its drafts from the root down, so its entries increase; it ends
+ * early at an entry that does not, or that is not in 0 .. n-1.
+ *   path  device int32 [batch, max_path], max_path <= n <= 256;  n_path, seq_len, new_len  device int32 [batch] */
+int nimllm_kv_accept(void *k_cache, void *v_cache, int cache_dtype, int n_layer, int64_t layer_stride,
+                     const int64_t *kv_off, int64_t seq_stride, int64_t head_stride, int max_seq, const int32_t *path,
+                     int max_path, const int32_t *n_path, const int32_t *seq_len, int32_t *new_len, int n, int batch,
+                     int n_kv_head, int head_dim, void *stream);
+int nimllm_kv_accept_paged(void *k_pages, void *v_pages, int cache_dtype, int n_layer, int64_t layer_stride,
+                           const int32_t *page_table, int max_pages, int page_rows, int n_pages, const int32_t *path,
+                           int max_path, const int32_t *n_path, const int32_t *seq_len, int32_t *new_len, int n, int batch,
+                           int n_kv_head, int head_dim, void *stream);
+
+/* nimllm_attn_decode (one token per sequence) that also keeps score of the cached rows:
+ *   score[b][h][r] = decay * score[b][h][r] + sum over the query heads of KV head h of the softmax weight of row r
+ * for r < seq_len[b]; score is device fp32 [batch][n_kv_head][score_rows], score_rows >= max_len; decay 0 does not
+ * read the old value.  head_dim 64 or 128; workspace as above. */
+size_t nimllm_attn_decode_scored_workspace_bytes(int batch, int n_head, int n_kv_head, int head_dim, int max_len,
+                                                 int cache_dtype);
+int nimllm_attn_decode_scored(const void *q, int q_dtype, const void *k_cache, const void *v_cache, int cache_dtype,
+                              const int64_t *kv_off, int64_t seq_stride, int64_t head_stride, int max_seq,
+                              const int32_t *seq_len, int max_len, void *out, int out_dtype, float *score,
+                              int64_t score_rows, float decay, int batch, int n_head, int n_kv_head, int head_dim,
+                              float scale, void *workspace, size_t workspace_bytes, void *stream);
+int nimllm_attn_decode_scored_paged(const void *q, int q_dtype, const void *k_pages, const void *v_pages, int cache_dtype,
+                                    const int32_t *page_table, int max_pages, int page_rows, int n_pages,
+                                    const int32_t *seq_len, int max_len, void *out, int out_dtype, float *score,
+                                    int64_t score_rows, float decay, int batch, int n_head, int n_kv_head, int head_dim,
+                                    float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Cuts every sequence longer than `keep` rows down to `keep`: in each KV head the first n_sink rows, the last n_recent
+ * and, of the others, those with the largest scores (of equal ones the lowest row; NaN counts as lowest) keep their
+ * order and move down; their scores move with them and the scores behind them become 0.
+ *   kept     device int32 [batch][n_kv_head][keep]: the former row of each kept one, -1 behind a shorter sequence
+ *   new_len  device int32 [batch] = min(seq_len, keep), may be seq_len (NULL seq_len: max_len rows each)
+ * K stays rotated at its old positions: append what follows with nimllm_rope_append_at. */
+int nimllm_kv_evict(void *k_cache, void *v_cache, int cache_dtype, const int64_t *kv_off, int64_t seq_stride,
+                    int64_t head_stride, int max_seq, float *score, int64_t score_rows, const int32_t *seq_len, int max_len,
+                    int keep, int n_sink, int n_recent, int32_t *kept, int32_t *new_len, int batch, int n_kv_head,
+                    int head_dim, void *stream);
+int nimllm_kv_evict_paged(void *k_pages, void *v_pages, int cache_dtype, const int32_t *page_table, int max_pages,
+                          int page_rows, int n_pages, float *score, int64_t score_rows, const int32_t *seq_len, int max_len,
+                          int keep, int n_sink, int n_recent, int32_t *kept, int32_t *new_len, int batch, int n_kv_head,
+                          int head_dim, void *stream);
 
 /* ---- GQA decode for callers that cannot allocate ------------------------------------
  * No counterpart in the reference.  Same computation and arguments as nimllm_attn_decode,

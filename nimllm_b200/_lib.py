@@ -10,11 +10,13 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnimllm_attn.so")
 
 F32, BF16 = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BASE, ROPE_SCALE_RAMP = 0, 1, 2, 3
 W_F32, W_BF16, W_Q8_0, W_Q4_0 = 0, 1, 2, 3
 
 _lib = None
 
-vp, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
+vp, i32, i64, f32, f64, sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double, C.c_size_t
 
 PROTOTYPES = {
     # name: (restype, argtypes)
@@ -38,6 +40,7 @@ PROTOTYPES = {
     "nimllm_kvpool_destroy": (None, [vp]),
     "nimllm_kvpool_reserve": (i32, [vp, i32, i32]),
     "nimllm_kvpool_release": (i32, [vp, i32]),
+    "nimllm_kvpool_shrink": (i32, [vp, i32, i32]),
     "nimllm_kvpool_sync": (i32, [vp, vp]),
     "nimllm_kvpool_free_pages": (i32, [vp]),
     "nimllm_kvpool_seq_pages": (i32, [vp, i32]),
@@ -52,6 +55,26 @@ PROTOTYPES = {
                                  i32, f32, i32, vp, sz, vp]),
     "nimllm_attn_decode_paged": (i32, [vp, i32, vp, vp, vp, i32, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, f32,
                                        vp, sz, vp]),
+    "nimllm_rope_tables_scaled_host": (i32, [vp, vp, i32, i32, f64, i32, f64, f64, f64, i32, f64]),
+    "nimllm_rope_append_at": (i32, [vp, vp, i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, vp, vp, i32, vp, vp, i32, vp, i64, i64,
+                                    i32, i32, i32, i32, i32, vp]),
+    "nimllm_rope_append_at_paged": (i32, [vp, vp, i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, vp, vp, i32, vp, vp, i32, vp, i32,
+                                          i32, i32, i32, i32, i32, i32, vp]),
+    "nimllm_rope_at_bwd": (i32, [vp, vp, i32, vp, vp, i32, vp, vp, i32, i32, i32, vp, i32, i32, i32, i32, i32, vp]),
+    "nimllm_attn_decode_tree_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
+    "nimllm_attn_decode_tree": (i32, [vp, i32, vp, vp, i32, vp, i64, i64, i32, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32,
+                                      i32, f32, vp, sz, vp]),
+    "nimllm_attn_decode_tree_paged": (i32, [vp, i32, vp, vp, i32, vp, i32, i32, i32, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32,
+                                            i32, i32, f32, vp, sz, vp]),
+    "nimllm_kv_accept": (i32, [vp, vp, i32, i32, i64, vp, i64, i64, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, vp]),
+    "nimllm_kv_accept_paged": (i32, [vp, vp, i32, i32, i64, vp, i32, i32, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, vp]),
+    "nimllm_attn_decode_scored_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+    "nimllm_attn_decode_scored": (i32, [vp, i32, vp, vp, i32, vp, i64, i64, i32, vp, i32, vp, i32, vp, i64, f32, i32, i32, i32,
+                                        i32, f32, vp, sz, vp]),
+    "nimllm_attn_decode_scored_paged": (i32, [vp, i32, vp, vp, i32, vp, i32, i32, i32, vp, i32, vp, i32, vp, i64, f32, i32, i32,
+                                              i32, i32, f32, vp, sz, vp]),
+    "nimllm_kv_evict": (i32, [vp, vp, i32, vp, i64, i64, i32, vp, i64, vp, i32, i32, i32, i32, vp, vp, i32, i32, i32, vp]),
+    "nimllm_kv_evict_paged": (i32, [vp, vp, i32, vp, i32, i32, i32, vp, i64, vp, i32, i32, i32, i32, vp, vp, i32, i32, i32, vp]),
     "nimllm_attn_decode_noalloc_max_bytes": (sz, []),
     "nimllm_attn_decode_noalloc": (i32, [vp, i32, vp, vp, i32, vp, i64, i64, vp, i32, vp, i32, vp, i32, i32, i32,
                                          i32, f32, i32, vp]),

@@ -130,6 +130,9 @@ class PagedKvPool:
     def release(self, seq: int):
         check(lib().nimllm_kvpool_release(self._h, seq))
 
+    def shrink(self, seq: int, rows_total: int):
+        check(lib().nimllm_kvpool_shrink(self._h, seq, rows_total))
+
     def sync(self):
         check(lib().nimllm_kvpool_sync(self._h, _stream() if self.on_device else None))
 
@@ -227,6 +230,335 @@ def rope_append_paged(q, k_new, v_new, cos, sin, k_pages, v_pages, page_table, *
         _ptr(q), n_head, _ptr(k_new), _ptr(v_new), _code(k_new), int(write_back_k), _ptr(cos), _ptr(sin),
         _ptr(seq_pos), pos0, _ptr(k_pages), _ptr(v_pages), _code(k_pages), _ptr(page_table), page_table.shape[1],
         k_pages.shape[2], k_pages.shape[0], B, n, n_kv_head, head_dim, _stream()))
+
+
+# ---- a cache whose rows are not its positions: drafted trees and evicted caches -------------------------------------
+_LAYOUT = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
+_SCALE_KIND = {"none": _lib.ROPE_SCALE_NONE, "linear": _lib.ROPE_SCALE_LINEAR, "base": _lib.ROPE_SCALE_BASE,
+               "ramp": _lib.ROPE_SCALE_RAMP}
+
+
+def _layout(name):
+    try:
+        return _LAYOUT[name]
+    except KeyError:
+        raise _lib.NimllmAttnError(f"unknown layout {name!r}: 'half' and 'interleaved' are built") from None
+
+
+def _args(device, dtypes, *tensors):
+    """Data pointers of contiguous tensors on one device, each of its dtype (None: any), which is the current one.
+    None stays None."""
+    ptrs = []
+    for t, dt in zip(tensors, dtypes):
+        if t is None:
+            ptrs.append(None)
+            continue
+        if t.device != device:
+            raise _lib.NimllmAttnError(f"tensors on {t.device} and on {device}")
+        if dt is not None and t.dtype != dt:
+            raise _lib.NimllmAttnError(f"{dt} tensor expected, got {t.dtype}")
+        ptrs.append(_ptr(t))
+    return ptrs
+
+
+def _sizes(**named):
+    """Every tensor holds at least the elements that its shape arguments say."""
+    for name, (t, least) in named.items():
+        if t is not None and t.numel() < least:
+            raise _lib.NimllmAttnError(f"{name} holds {t.numel()} elements, {least} are needed")
+
+
+def _block_sizes(k_cache, v_cache, kv_off, batch, n_kv_head, head_dim, seq_stride, head_stride, max_seq, layers=0, layer_stride=0):
+    """Without kv_off the blocks' ends are known: they have to lie in the tensors."""
+    if kv_off is not None or max_seq <= 0:
+        return
+    end = max(layers - 1, 0) * layer_stride + (batch - 1) * seq_stride + (n_kv_head - 1) * head_stride + max_seq * head_dim
+    _sizes(k_cache=(k_cache, end), v_cache=(v_cache, end))
+
+
+def _on(device):
+    """The context in which a call for tensors of `device` launches."""
+    if device.type != "cuda":
+        raise _lib.NimllmAttnError("device tensor expected (there is no CPU path)")
+    return _same if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+class _Same:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *a):
+        pass
+
+
+_same = _Same()
+
+
+def _scratch(nbytes, device):
+    # from the caching allocator of the current stream, so calls on two streams or in two graphs never share it
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def rope_tables_scaled(max_pos: int, rot_dim: int, base: float, *, kind="none", factor=1.0, low=1.0, high=32.0, orig_len=0,
+                       gain=1.0, device="cuda"):
+    """cos/sin tables [max_pos, rot_dim/2] for positions past the trained length: kind "linear" divides every frequency
+    by factor, "base" stretches the base, "ramp" interpolates between both by the turns a frequency makes over orig_len
+    positions (kept at `high` turns and more, divided at `low` and fewer)."""
+    cos = np.empty((max_pos, rot_dim // 2), np.float32)
+    sin = np.empty_like(cos)
+    if kind not in _SCALE_KIND:
+        raise _lib.NimllmAttnError(f"unknown kind {kind!r}: {sorted(_SCALE_KIND)} are built")
+    check(lib().nimllm_rope_tables_scaled_host(cos.ctypes.data, sin.ctypes.data, max_pos, rot_dim, float(base), _SCALE_KIND[kind],
+                                               float(factor), float(low), float(high), int(orig_len), float(gain)))
+    return torch.from_numpy(cos).to(device), torch.from_numpy(sin).to(device)
+
+
+def _rope_at(q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out, k_out, want_k, has_cache):
+    if k_new is None:
+        raise _lib.NimllmAttnError("k_new is required")
+    B, n = k_new.shape[0], k_new.shape[1]
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q)
+    if k_out is None and (want_k or not has_cache):
+        k_out = torch.empty_like(k_new)
+    act, kv = k_new.dtype, B * n * n_kv_head * head_dim
+    qs = B * n * n_head * head_dim
+    _sizes(q=(q, qs), q_out=(q_out, qs), k_new=(k_new, kv), k_out=(k_out, kv), v_new=(v_new, kv), pos=(pos, B * n), row0=(row0, B))
+    if cos is not None and sin is not None and cos.shape != sin.shape:
+        raise _lib.NimllmAttnError("cos and sin differ in shape")
+    p = _args(k_new.device, (act, act, None, act, act, torch.float32, torch.float32, torch.int32, torch.int32),
+              q, q_out, k_new, k_out, v_new, cos, sin, pos, row0)
+    rot, rows = (2 * cos.shape[1], cos.shape[0]) if cos is not None else (0, 0)
+    head = (p[0], p[1], n_head, p[2], p[3], p[4], _code(k_new), p[5], p[6], rot, _layout(layout), rows, p[7], p[8])
+    return B, n, q_out if q is not None else None, k_out, head
+
+
+def rope_append_at(q, k_new, v_new, cos, sin, *, n_head, n_kv_head, head_dim, layout="half", pos=None, row0=None, first_row=0,
+                   k_cache=None, v_cache=None, kv_off=None, seq_stride=0, head_stride=0, max_seq=0, q_out=None, k_out=None,
+                   want_k=False):
+    """Rotates q and k_new [B, n, heads*D] at pos [B, n] (int32; negative: padding, left alone) and appends k and v at the
+    rows row0[b] + t.  cos/sin [rows, R/2] rotate the first R columns of every head.  Returns (q_out, k_out)."""
+    with _on(k_new.device):
+        B, n, q_out, k_out, head = _rope_at(q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out, k_out,
+                                            want_k, k_cache is not None)
+        if k_cache is not None:
+            _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
+        kc, vc, off = _args(k_new.device, (None, k_cache.dtype if k_cache is not None else None, torch.int64), k_cache, v_cache, kv_off)
+        check(lib().nimllm_rope_append_at(*head, first_row, kc, vc, _code(k_cache) if k_cache is not None else F32, off, seq_stride,
+                                          head_stride, max_seq, B, n, n_kv_head, head_dim, _stream()))
+    return q_out, k_out
+
+
+def _pages(k_pages, v_pages, page_table, batch, n_kv_head, head_dim, layers=None):
+    """(n_pages, page_rows) of pages [(layers,) n_pages, Hkv, page_rows, D], checked against the heads and the table."""
+    want = k_pages.shape[-4:]
+    if k_pages.dim() not in (4, 5) or want[1] != n_kv_head or want[3] != head_dim or v_pages.shape != k_pages.shape:
+        raise _lib.NimllmAttnError(f"pages {tuple(k_pages.shape)} / {tuple(v_pages.shape)}: [n_pages, {n_kv_head}, page_rows, {head_dim}] expected")
+    if (k_pages.shape[0] if k_pages.dim() == 5 else 1) < (layers or 1):
+        raise _lib.NimllmAttnError(f"pages {tuple(k_pages.shape)}: {layers} layers expected")
+    if page_table.dim() != 2 or page_table.shape[0] < batch:
+        raise _lib.NimllmAttnError(f"page_table {tuple(page_table.shape)}: [{batch}, max_pages] expected")
+    return want[0], want[2]
+
+
+def rope_append_at_paged(q, k_new, v_new, cos, sin, k_pages, v_pages, page_table, *, n_head, n_kv_head, head_dim, layout="half",
+                         pos=None, row0=None, first_row=0, q_out=None, k_out=None, want_k=False):
+    """rope_append_at into pages [n_pages, Hkv, page_rows, D] with page_table int32 [B, max_pages]."""
+    with _on(k_new.device):
+        B, n, q_out, k_out, head = _rope_at(q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out, k_out,
+                                            want_k, True)
+        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        kp, vp, pt = _args(k_new.device, (None, k_pages.dtype, torch.int32), k_pages, v_pages, page_table)
+        check(lib().nimllm_rope_append_at_paged(*head, first_row, kp, vp, _code(k_pages), pt, page_table.shape[1], page_rows, n_pages,
+                                                B, n, n_kv_head, head_dim, _stream()))
+    return q_out, k_out
+
+
+def rope_at_backward(dq_rot, dk_rot, cos, sin, *, n_head, n_kv_head, head_dim, layout="half", pos=None, pos0=0, in_place=False):
+    """Gradient of the rotation: (dq, dk) from the gradients of the rotated q and k [B, n, heads*D] (either may be None).
+    Tokens without a position get zeros."""
+    some = dq_rot if dq_rot is not None else dk_rot
+    if some is None:
+        raise _lib.NimllmAttnError("dq_rot or dk_rot is required")
+    B, n = some.shape[0], some.shape[1]
+    with _on(some.device):
+        dq = dq_rot if in_place or dq_rot is None else torch.empty_like(dq_rot)
+        dk = dk_rot if in_place or dk_rot is None else torch.empty_like(dk_rot)
+        _sizes(dq_rot=(dq_rot, B * n * n_head * head_dim), dk_rot=(dk_rot, B * n * n_kv_head * head_dim), pos=(pos, B * n))
+        if cos.shape != sin.shape:
+            raise _lib.NimllmAttnError("cos and sin differ in shape")
+        dt = some.dtype
+        p = _args(some.device, (dt, dt, dt, dt, torch.float32, torch.float32, torch.int32), dq_rot, dq, dk_rot, dk, cos, sin, pos)
+        check(lib().nimllm_rope_at_bwd(p[0], p[1], n_head, p[2], p[3], _code(some), p[4], p[5], 2 * cos.shape[1], _layout(layout),
+                                       cos.shape[0], p[6], pos0, B, n, n_kv_head, head_dim, _stream()))
+    return dq, dk
+
+
+def _tree_io(q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim):
+    B, n = q.shape[0], q.shape[1]
+    if out is None:
+        # with n_new the rows of padding tokens are not written
+        out = (torch.empty if n_new is None else torch.zeros)((B, n, n_head * head_dim), dtype=out_dtype, device=q.device)
+    rec = torch.empty((B * n * n_head, head_dim + 4), dtype=torch.float32, device=q.device) if partials else None
+    size = B * n * n_head * head_dim
+    _sizes(q=(q, size), out=(out, size), n_new=(n_new, B), tree_mask=(tree_mask, B * n * ((n + 63) // 64)), seq_len=(seq_len, B))
+    return B, n, out, rec
+
+
+def decode_tree(q, k_cache, v_cache, *, n_head, n_kv_head, head_dim, max_len, max_seq, seq_len=None, n_new=None, tree_mask=None,
+                kv_off=None, seq_stride=0, head_stride=0, scale=None, out=None, out_dtype=torch.float32, partials=False):
+    """Attention of the drafted tokens q [B, n, Hq*D]: token i of sequence b attends its seq_len[b] committed rows and the
+    draft rows seq_len[b] + j with bit j set in tree_mask [B, n, ceil(n/64)] (int64; None: drafts 0 .. i).  Returns out
+    [B, n, Hq*D] (and the (o, m, l) records [B*n*Hq, D+4] when partials=True)."""
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+    with _on(q.device):
+        B, n, out, rec = _tree_io(q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim)
+        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
+        p = _args(q.device, (None, None, k_cache.dtype, torch.int64, torch.int32, torch.int32, torch.int64, None),
+                  q, k_cache, v_cache, kv_off, seq_len, n_new, tree_mask, out)
+        code = _code(k_cache)
+        need = lib().nimllm_attn_decode_tree_workspace_bytes(B, n, n_head, n_kv_head, head_dim, max_len, code)
+        ws = _scratch(need, q.device)
+        check(lib().nimllm_attn_decode_tree(
+            p[0], _code(q), p[1], p[2], code, p[3], seq_stride, head_stride, max_seq, p[4], max_len, p[5], p[6], p[7], _code(out),
+            _ptr(rec), B, n, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+    return (out, rec) if partials else out
+
+
+def decode_tree_paged(q, k_pages, v_pages, page_table, *, n_head, n_kv_head, head_dim, max_len, seq_len=None, n_new=None,
+                      tree_mask=None, scale=None, out=None, out_dtype=torch.float32, partials=False):
+    """decode_tree over pages [n_pages, Hkv, page_rows, D] with page_table int32 [B, max_pages]."""
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+    with _on(q.device):
+        B, n, out, rec = _tree_io(q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim)
+        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        p = _args(q.device, (None, None, k_pages.dtype, torch.int32, torch.int32, torch.int32, torch.int64, None),
+                  q, k_pages, v_pages, page_table, seq_len, n_new, tree_mask, out)
+        code = _code(k_pages)
+        need = lib().nimllm_attn_decode_tree_workspace_bytes(B, n, n_head, n_kv_head, head_dim, max_len, code)
+        ws = _scratch(need, q.device)
+        check(lib().nimllm_attn_decode_tree_paged(
+            p[0], _code(q), p[1], p[2], code, p[3], page_table.shape[1], page_rows, n_pages, p[4], max_len, p[5], p[6], p[7],
+            _code(out), _ptr(rec), B, n, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+    return (out, rec) if partials else out
+
+
+def _accept_io(path, n_path, seq_len, new_len):
+    B, max_path = path.shape
+    new_len = torch.empty_like(seq_len) if new_len is None else new_len
+    _sizes(n_path=(n_path, B), seq_len=(seq_len, B), new_len=(new_len, B))
+    i = torch.int32
+    return B, max_path, new_len, _args(path.device, (i, i, i, i), path, n_path, seq_len, new_len)
+
+
+def kv_accept(k_cache, v_cache, path, n_path, seq_len, *, n_draft, n_kv_head, head_dim, max_seq, n_layer=1, layer_stride=0,
+              kv_off=None, seq_stride=0, head_stride=0, new_len=None):
+    """Moves the rows of the accepted drafts path[b][:n_path[b]] (int32 [B, max_path], increasing) down to the rows from
+    seq_len[b] on, in n_layer layers, and returns new_len [B] (given: written there; it may be seq_len)."""
+    with _on(path.device):
+        B, max_path, new_len, p = _accept_io(path, n_path, seq_len, new_len)
+        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq, n_layer, layer_stride)
+        kc, vc, off = _args(path.device, (None, k_cache.dtype, torch.int64), k_cache, v_cache, kv_off)
+        check(lib().nimllm_kv_accept(kc, vc, _code(k_cache), n_layer, layer_stride, off, seq_stride, head_stride, max_seq, p[0],
+                                     max_path, p[1], p[2], p[3], n_draft, B, n_kv_head, head_dim, _stream()))
+    return new_len
+
+
+def kv_accept_paged(k_pages, v_pages, page_table, path, n_path, seq_len, *, n_draft, n_kv_head, head_dim, n_layer=1, new_len=None):
+    """kv_accept over pages [(n_layer,) n_pages, Hkv, page_rows, D]; all layers share the page table."""
+    with _on(path.device):
+        B, max_path, new_len, p = _accept_io(path, n_path, seq_len, new_len)
+        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim, n_layer)
+        kp, vp, pt = _args(path.device, (None, k_pages.dtype, torch.int32), k_pages, v_pages, page_table)
+        check(lib().nimllm_kv_accept_paged(kp, vp, _code(k_pages), n_layer, n_pages * n_kv_head * page_rows * head_dim, pt,
+                                           page_table.shape[1], page_rows, n_pages, p[0], max_path, p[1], p[2], p[3], n_draft, B,
+                                           n_kv_head, head_dim, _stream()))
+    return new_len
+
+
+def _scored_io(q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim):
+    B = q.shape[0]
+    if score.dim() != 3 or score.shape[0] < B or score.shape[1] != n_kv_head:
+        raise _lib.NimllmAttnError(f"score {tuple(score.shape)}: [{B}, {n_kv_head}, rows] expected")
+    if out is None:
+        out = torch.empty((B, n_head * head_dim), dtype=out_dtype, device=q.device)
+    _sizes(q=(q, B * n_head * head_dim), out=(out, B * n_head * head_dim), seq_len=(seq_len, B))
+    return B, out
+
+
+def decode_scored(q, k_cache, v_cache, score, *, n_head, n_kv_head, head_dim, max_len, max_seq, seq_len=None, decay=1.0, kv_off=None,
+                  seq_stride=0, head_stride=0, scale=None, out=None, out_dtype=torch.float32):
+    """decode_batch that also updates score [B, Hkv, rows] (fp32): decay * score + the softmax weights of the query heads
+    of each KV head, summed.  Returns out [B, Hq*D]."""
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+    with _on(q.device):
+        B, out = _scored_io(q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim)
+        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
+        p = _args(q.device, (None, None, k_cache.dtype, torch.int64, torch.int32, None, torch.float32),
+                  q, k_cache, v_cache, kv_off, seq_len, out, score)
+        code = _code(k_cache)
+        need = lib().nimllm_attn_decode_scored_workspace_bytes(B, n_head, n_kv_head, head_dim, max_len, code)
+        ws = _scratch(need, q.device)
+        check(lib().nimllm_attn_decode_scored(
+            p[0], _code(q), p[1], p[2], code, p[3], seq_stride, head_stride, max_seq, p[4], max_len, p[5], _code(out), p[6],
+            score.shape[2], decay, B, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+    return out
+
+
+def decode_scored_paged(q, k_pages, v_pages, page_table, score, *, n_head, n_kv_head, head_dim, max_len, seq_len=None, decay=1.0,
+                        scale=None, out=None, out_dtype=torch.float32):
+    """decode_scored over pages [n_pages, Hkv, page_rows, D] with page_table int32 [B, max_pages]."""
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+    with _on(q.device):
+        B, out = _scored_io(q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim)
+        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        p = _args(q.device, (None, None, k_pages.dtype, torch.int32, torch.int32, None, torch.float32),
+                  q, k_pages, v_pages, page_table, seq_len, out, score)
+        code = _code(k_pages)
+        need = lib().nimllm_attn_decode_scored_workspace_bytes(B, n_head, n_kv_head, head_dim, max_len, code)
+        ws = _scratch(need, q.device)
+        check(lib().nimllm_attn_decode_scored_paged(
+            p[0], _code(q), p[1], p[2], code, p[3], page_table.shape[1], page_rows, n_pages, p[4], max_len, p[5], _code(out), p[6],
+            score.shape[2], decay, B, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+    return out
+
+
+def _evict_io(score, seq_len, keep, kept, new_len, n_kv_head, batch):
+    B = score.shape[0] if batch is None else batch
+    if score.dim() != 3 or score.shape[0] < B or score.shape[1] != n_kv_head:
+        raise _lib.NimllmAttnError(f"score {tuple(score.shape)}: [{B}, {n_kv_head}, rows] expected")
+    if kept is None:
+        kept = torch.empty((B, n_kv_head, max(keep, 0)), dtype=torch.int32, device=score.device)
+    if new_len is None:
+        new_len = torch.empty(B, dtype=torch.int32, device=score.device)
+    _sizes(seq_len=(seq_len, B), kept=(kept, B * n_kv_head * keep), new_len=(new_len, B))
+    i = torch.int32
+    return B, kept, new_len, _args(score.device, (torch.float32, i, i, i), score, seq_len, kept, new_len)
+
+
+def kv_evict(k_cache, v_cache, score, seq_len, *, keep, n_kv_head, head_dim, max_len, max_seq, n_sink=0, n_recent=0, kv_off=None,
+             seq_stride=0, head_stride=0, kept=None, new_len=None, batch=None):
+    """Cuts every sequence to `keep` rows: per KV head the first n_sink, the last n_recent and those with the largest
+    score [B, Hkv, rows] in between, in order; K, V and score move.  Returns (new_len [B], kept [B, Hkv, keep])."""
+    with _on(score.device):
+        B, kept, new_len, p = _evict_io(score, seq_len, keep, kept, new_len, n_kv_head, batch)
+        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
+        kc, vc, off = _args(score.device, (None, k_cache.dtype, torch.int64), k_cache, v_cache, kv_off)
+        check(lib().nimllm_kv_evict(kc, vc, _code(k_cache), off, seq_stride, head_stride, max_seq, p[0], score.shape[2], p[1], max_len,
+                                    keep, n_sink, n_recent, p[2], p[3], B, n_kv_head, head_dim, _stream()))
+    return new_len, kept
+
+
+def kv_evict_paged(k_pages, v_pages, page_table, score, seq_len, *, keep, n_kv_head, head_dim, max_len, n_sink=0, n_recent=0, kept=None,
+                   new_len=None, batch=None):
+    """kv_evict over pages [n_pages, Hkv, page_rows, D]; give the empty pages back with PagedKvPool.shrink."""
+    with _on(score.device):
+        B, kept, new_len, p = _evict_io(score, seq_len, keep, kept, new_len, n_kv_head, batch)
+        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        kp, vp, pt = _args(score.device, (None, k_pages.dtype, torch.int32), k_pages, v_pages, page_table)
+        check(lib().nimllm_kv_evict_paged(kp, vp, _code(k_pages), pt, page_table.shape[1], page_rows, n_pages, p[0], score.shape[2], p[1],
+                                          max_len, keep, n_sink, n_recent, p[2], p[3], B, n_kv_head, head_dim, _stream()))
+    return new_len, kept
 
 
 def _wtype(w, w_type):

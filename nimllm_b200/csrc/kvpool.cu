@@ -106,6 +106,21 @@ int nimllm_kvpool_release(nimllm_kvpool *p, int seq) {
     return NIMLLM_OK;
 }
 
+/* Gives the pages past the first rows_total rows back (an eviction or drafts that were not accepted left them empty). */
+int nimllm_kvpool_shrink(nimllm_kvpool *p, int seq, int rows_total) {
+    if (!p || seq < 0 || seq >= p->max_seqs || rows_total < 0) return fail(NIMLLM_ERR_ARG, "kvpool_shrink: bad arguments");
+    if (rows_total >= p->rows[seq]) return NIMLLM_OK;
+    const int need = (int)(((int64_t)rows_total + p->page_rows - 1) / p->page_rows);
+    for (; p->n_held[seq] > need; p->n_held[seq]--) {
+        int32_t &e = p->table[(size_t)seq * p->max_pages + p->n_held[seq] - 1];
+        p->free_list.push_back(e);
+        e = -1;
+        p->dirty[seq] = 1;
+    }
+    p->rows[seq] = rows_total;
+    return NIMLLM_OK;
+}
+
 /* Uploads the table rows that changed since the last call (one cudaMemcpyAsync per changed sequence,
  * from the pool's own host copy: call it before the launches that read the table, on their stream). */
 int nimllm_kvpool_sync(nimllm_kvpool *p, void *stream) {

@@ -1,0 +1,199 @@
+"""CPU tests of the operators on a cache whose rows are not its positions: refusals, scaled tables, pages given back."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from nimllm_b200 import _lib
+from nimllm_b200 import attention as A
+
+L = _lib.lib()
+P = C.c_void_p(256)
+
+
+def refused(rc, code, word):
+    assert rc == code and word.encode() in L.nimllm_attn_last_error(), (rc, L.nimllm_attn_last_error())
+
+
+def _rope(**o):
+    a = dict(q=P, q_out=P, Hq=4, k=P, k_out=P, v=P, act=0, cos=P, sin=P, rot=64, layout=0, rows=16, pos=None, row0=None, first=0,
+             kc=P, vc=P, cache=0, off=None, ss=4096, hs=2048, cap=32, B=1, n=1, Hkv=2, D=64, st=None)
+    a.update(o)
+    return L.nimllm_rope_append_at(*a.values())
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(cos=None), 1, "both RoPE tables"), (dict(q_out=None), 1, "q and q_out"), (dict(vc=None), 1, "both cache pointers"),
+    (dict(k=None), 1, "k_new"), (dict(v=None), 1, "v_new"), (dict(rot=60), 1, "rot_dim"), (dict(rot=72), 1, "rot_dim"), (dict(rot=0), 1, "rot_dim"),
+    (dict(rows=0), 1, "table_rows"), (dict(layout=2), 1, "layout"), (dict(act=2), 1, "dtype"), (dict(cache=7), 1, "dtype"), (dict(D=60), 1, "bad shape"),
+    (dict(hs=2050), 1, "multiples of 16"), (dict(cap=0), 1, "max_seq"), (dict(q=C.c_void_p(8)), 1, "aligned"), (dict(kc=C.c_void_p(24)), 1, "aligned"),
+    (dict(cos=C.c_void_p(4)), 1, "aligned"), (dict(n=-1), 1, "bad shape")])
+def test_rope_at_refusals(change, code, word):
+    refused(_rope(**change), code, word)
+
+
+def test_rope_at_of_nothing():
+    assert _rope(n=0) == 0 and _rope(B=0) == 0
+
+
+def test_rope_at_bwd_refusals():
+    f = L.nimllm_rope_at_bwd
+    refused(f(P, P, 4, P, P, 0, None, P, 64, 0, 16, None, 0, 1, 1, 2, 64, None), 1, "tables")
+    refused(f(P, None, 4, P, P, 0, P, P, 64, 0, 16, None, 0, 1, 1, 2, 64, None), 1, "gradient")
+    refused(f(None, None, 4, None, None, 0, P, P, 64, 0, 16, None, 0, 1, 1, 2, 64, None), 1, "gradient")
+    refused(f(P, C.c_void_p(8), 4, P, P, 0, P, P, 64, 0, 16, None, 0, 1, 1, 2, 64, None), 1, "aligned")
+
+
+def _tree(**o):
+    a = dict(q=P, qt=0, k=P, v=P, ct=1, off=None, ss=65536, hs=16384, cap=128, len=None, max_len=100, n_new=None, mask=None, out=P, ot=0, rec=None,
+             B=1, n=4, Hq=4, Hkv=2, D=64, scale=0.125, ws=None, bytes=0, st=None)
+    a.update(o)
+    return L.nimllm_attn_decode_tree(*a.values())
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(q=None), 1, "null"), (dict(out=None), 1, "null"), (dict(k=None), 1, "null cache"), (dict(Hq=5), 1, "bad shape"), (dict(n=0), 1, "bad shape"),
+    (dict(max_len=-1), 1, "bad shape"), (dict(n=257), 2, "257"), (dict(D=96), 2, "head_dim"), (dict(qt=3), 1, "dtype"), (dict(ct=2), 1, "dtype"), (dict(cap=0), 1, "max_seq"),
+    (dict(hs=16386), 1, "multiples of 16"), (dict(ss=3), 1, "multiples of 16"), (dict(mask=C.c_void_p(12)), 1, "8-byte"), (dict(B=70000), 2, "too large"),
+    (dict(out=C.c_void_p(8)), 1, "aligned")])
+def test_tree_refusals(change, code, word):
+    refused(_tree(**change), code, word)
+
+
+def test_workspaces_are_asked_for():
+    need = L.nimllm_attn_decode_tree_workspace_bytes(4, 8, 32, 8, 128, 100000, 0)
+    assert need > 0
+    refused(_tree(ct=0, B=4, n=8, Hq=32, Hkv=8, D=128, max_len=100000), 3, "workspace")
+    refused(_tree(ct=0, B=4, n=8, Hq=32, Hkv=8, D=128, max_len=100000, ws=P, bytes=need - 1), 3, "workspace")
+    refused(_tree(ct=0, B=4, n=8, Hq=32, Hkv=8, D=128, max_len=100000, ws=C.c_void_p(264), bytes=need), 1, "256-byte")
+    assert L.nimllm_attn_decode_scored_workspace_bytes(1, 4, 2, 64, 100, 1) >= 4 * 128 * 4
+    assert L.nimllm_attn_decode_scored_workspace_bytes(0, 4, 2, 64, 100, 1) == 0
+    assert L.nimllm_attn_decode_tree_workspace_bytes(1, 300, 4, 2, 64, 100, 1) == 0
+
+
+def test_paged_refusals():
+    f = L.nimllm_attn_decode_tree_paged
+    tail = (None, 100, None, None, P, 0, None, 1, 4, 4, 2, 64, 0.125, None, 0, None)
+    refused(f(P, 0, P, P, 1, None, 4, 32, 9, *tail), 1, "null pages")
+    refused(f(P, 0, P, P, 1, P, 4, 48, 9, *tail), 1, "page_rows")
+    refused(f(P, 0, P, P, 1, P, 4, 16, 9, *tail), 1, "page_rows")
+    refused(f(P, 0, P, P, 1, P, 0, 32, 9, *tail), 1, "max_pages")
+    refused(f(P, 0, P, P, 1, P, 4, 32, 0, *tail), 1, "n_pages")
+    refused(f(P, 0, C.c_void_p(8), P, 1, P, 4, 32, 9, *tail), 1, "aligned")
+    refused(f(P, 0, P, P, 1, P, 2**30, 32, 9, *tail), 1, "max_pages")
+
+
+def test_scored_refusals():
+    f = L.nimllm_attn_decode_scored
+
+    def go(**o):
+        a = dict(q=P, qt=0, k=P, v=P, ct=1, off=None, ss=65536, hs=16384, cap=128, len=None, max_len=100, out=P, ot=0, score=P, rows=100, decay=1.0,
+                 B=1, Hq=4, Hkv=2, D=64, scale=0.125, ws=None, bytes=0, st=None)
+        a.update(o)
+        return f(*a.values())
+    refused(go(score=None), 1, "score")
+    refused(go(rows=99), 1, "99 scores")
+    refused(go(max_len=0), 1, "max_len")
+    refused(go(D=32), 2, "head_dim")
+    refused(go(), 3, "workspace")
+
+
+def test_accept_refusals():
+    f = L.nimllm_kv_accept
+
+    def go(**o):
+        a = dict(k=P, v=P, ct=1, L=2, ls=1 << 20, off=None, ss=65536, hs=16384, cap=128, path=P, mp=4, np=P, len=P, new=P, n=8, B=1, Hkv=2, D=64, st=None)
+        a.update(o)
+        return f(*a.values())
+    refused(go(path=None), 1, "null path")
+    refused(go(new=None), 1, "null path")
+    refused(go(mp=9), 2, "max_path")
+    refused(go(n=257, mp=4), 2, "n 257")
+    refused(go(mp=0), 1, "bad shape")
+    refused(go(L=0), 1, "bad shape")
+    refused(go(ls=12), 1, "layer_stride")
+    refused(go(D=60), 2, "16 bytes")
+
+
+def test_evict_refusals():
+    f = L.nimllm_kv_evict
+
+    def go(**o):
+        a = dict(k=P, v=P, ct=1, off=None, ss=65536, hs=16384, cap=128, score=P, rows=128, len=P, max_len=128, keep=64, sink=4, recent=8, kept=P, new=P,
+                 B=1, Hkv=2, D=64, st=None)
+        a.update(o)
+        return f(*a.values())
+    refused(go(score=None), 1, "null score")
+    refused(go(kept=None), 1, "null score")
+    refused(go(keep=0), 1, "keep")
+    refused(go(sink=60), 1, "keep")
+    refused(go(sink=-1), 1, "keep")
+    refused(go(recent=2**31 - 1), 1, "keep")
+    refused(go(max_len=129), 1, "holds 128 rows")
+    refused(go(rows=100), 1, "100 scores")
+
+
+def test_python_checks_shapes_before_anything_runs():
+    t = torch.zeros(1, 4, 256)
+    with pytest.raises(_lib.NimllmAttnError, match="device tensor"):
+        A.decode_tree(t, t, t, n_head=4, n_kv_head=2, head_dim=64, max_len=4, max_seq=8)
+    with pytest.raises(_lib.NimllmAttnError, match="device tensor"):
+        A.rope_append_at(t, t, t, None, None, n_head=4, n_kv_head=4, head_dim=64)
+
+
+def _freqs(rot, base):
+    return base ** (-2.0 * np.arange(rot // 2) / rot)
+
+
+@pytest.mark.parametrize("kind,factor", [("none", 1.0), ("linear", 8.0), ("base", 4.0), ("ramp", 16.0)])
+def test_scaled_tables(kind, factor):
+    rot, base, rows, orig, low, high, gain = 64, 10000.0, 5000, 2048, 1.0, 32.0, 1.1
+    cos, sin = A.rope_tables_scaled(rows, rot, base, kind=kind, factor=factor, low=low, high=high, orig_len=orig, gain=gain, device="cpu")
+    w = _freqs(rot, base)
+    if kind == "linear":
+        w = w / factor
+    elif kind == "base":
+        w = _freqs(rot, base * factor ** (rot / (rot - 2)))
+        assert abs(w[-1] * factor / _freqs(rot, base)[-1] - 1) < 1e-12
+    elif kind == "ramp":
+        t = orig * w / (2 * math.pi)
+        keep = np.clip((t - low) / (high - low), 0, 1)
+        assert keep.max() == 1 and keep.min() == 0
+        w = w * keep + w / factor * (1 - keep)
+    angle = np.arange(rows)[:, None] * w[None]
+    # half a step of the table's type, and 2^-40 for angles computed in another order
+    for got, want in ((cos, gain * np.cos(angle)), (sin, gain * np.sin(angle))):
+        assert (np.abs(got.numpy().astype(np.float64) - want) <= 2.0 ** -24 * np.abs(want) + 2.0 ** -40 * gain).all()
+
+
+def test_scaled_tables_refusals():
+    c = np.zeros((4, 32), np.float32)
+    f = lambda **o: L.nimllm_rope_tables_scaled_host(*{**dict(c=c.ctypes.data, s=c.ctypes.data, n=4, rot=64, base=1e4, kind=1, factor=2.0, low=1.0, high=4.0, orig=8, gain=1.0), **o}.values())
+    assert f() == 0
+    for bad in (dict(c=None), dict(rot=63), dict(base=-1.0), dict(kind=4), dict(factor=0.0), dict(kind=2, rot=2), dict(kind=3, low=4.0), dict(kind=3, orig=0), dict(factor=float("nan"))):
+        assert f(**bad) == 1
+    with pytest.raises(_lib.NimllmAttnError, match="unknown kind"):
+        A.rope_tables_scaled(4, 64, 1e4, kind="twice", device="cpu")
+
+
+def test_pool_shrink_gives_pages_back():
+    pool = A.PagedKvPool(1, 10, 32, 1, 64, 2, 8, on_device=False)
+    pool.reserve(0, 200)
+    pool.reserve(1, 33)
+    before = pool.table_host()
+    pool.shrink(0, 65)
+    t = pool.table_host()
+    assert pool.free_pages == 10 - 3 - 2 and pool.seq_pages(0) == 3 and pool.seq_rows(0) == 65
+    assert (t[0, :3] == before[0, :3]).all() and (t[0, 3:] == -1).all() and (t[1] == before[1]).all()
+    pool.shrink(0, 400)                       # more than it holds: nothing changes
+    assert pool.seq_rows(0) == 65
+    pool.reserve(1, 7 * 32)
+    assert pool.free_pages == 0
+    assert len({x for x in pool.table_host().flatten().tolist() if x >= 0}) == 10
+    pool.shrink(0, 0)
+    assert pool.seq_pages(0) == 0 and pool.free_pages == 3
+    for seq, rows in ((-1, 0), (2, 0), (0, -1)):
+        with pytest.raises(_lib.NimllmAttnError):
+            pool.shrink(seq, rows)
