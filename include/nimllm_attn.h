@@ -278,7 +278,10 @@ int nimllm_rope_at_bwd(const void *dq_rot, void *dq, int n_head, const void *dk_
  *   partials_out  optional fp32 [batch*n*n_head, head_dim + 4] records as in nimllm_attn_decode (out may be NULL then)
  *   head_dim   64 or 128.  The products are those of 32-bit arithmetic for either cache type; every row of V up to the last
  *              draft must be finite even where a mask hides it (a hidden row of K may hold anything)
- *   workspace  256-byte aligned, nimllm_attn_decode_tree_workspace_bytes(...) bytes */
+ *   workspace  256-byte aligned, nimllm_attn_decode_tree_workspace_bytes(...) bytes
+ * The kernel for bf16 caches (also that of nimllm_attn_decode_scored) bounds its internal waits, about 2 s without
+ * progress; nimllm_attn_decode_tree_status tells as nimllm_attn_prefill_status does whether one gave up. */
+int nimllm_attn_decode_tree_status(int reset);
 size_t nimllm_attn_decode_tree_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, int max_len,
                                                int cache_dtype);
 int nimllm_attn_decode_tree(const void *q, int q_dtype, const void *k_cache, const void *v_cache, int cache_dtype,

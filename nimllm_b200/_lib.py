@@ -61,6 +61,7 @@ PROTOTYPES = {
     "nimllm_rope_append_at_paged": (i32, [vp, vp, i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, vp, vp, i32, vp, vp, i32, vp, i32,
                                           i32, i32, i32, i32, i32, i32, vp]),
     "nimllm_rope_at_bwd": (i32, [vp, vp, i32, vp, vp, i32, vp, vp, i32, i32, i32, vp, i32, i32, i32, i32, i32, vp]),
+    "nimllm_attn_decode_tree_status": (i32, [i32]),
     "nimllm_attn_decode_tree_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
     "nimllm_attn_decode_tree": (i32, [vp, i32, vp, vp, i32, vp, i64, i64, i32, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32,
                                       i32, f32, vp, sz, vp]),

@@ -443,6 +443,15 @@ def decode_tree_paged(q, k_pages, v_pages, page_table, *, n_head, n_kv_head, hea
     return (out, rec) if partials else out
 
 
+def decode_tree_status(reset: bool = True) -> int:
+    """0 when every tree and scored decode over a bf16 cache on the current device since the last reset ran to completion,
+    1 when a bounded wait inside one gave up (its outputs are incomplete).  Synchronises."""
+    rc = lib().nimllm_attn_decode_tree_status(int(reset))
+    if rc < 0:
+        check(-rc)
+    return rc
+
+
 def _accept_io(path, n_path, seq_len, new_len):
     B, max_path = path.shape
     new_len = torch.empty_like(seq_len) if new_len is None else new_len

@@ -235,9 +235,10 @@ size_t fma_record_bytes(int batch, int n, int n_head, int n_kv_head, int head_di
     return chunks <= 1 ? 0 : (size_t)chunks * batch * n * n_head * rec_stride(head_dim) * sizeof(float);
 }
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
-bool use_tensor_cores(int cache_dtype) { (void)cache_dtype; return false; }
+bool use_tensor_cores(int cache_dtype) { return cache_dtype == NIMLLM_BF16; }
 size_t record_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, int max_total, int cache_dtype) {
-    return round256(use_tensor_cores(cache_dtype) ? 0 : fma_record_bytes(batch, n, n_head, n_kv_head, head_dim, max_total));
+    return round256(use_tensor_cores(cache_dtype) ? tree_tc_workspace_bytes(batch, n, n_head, n_kv_head, head_dim)
+                                                    : fma_record_bytes(batch, n, n_head, n_kv_head, head_dim, max_total));
 }
 int64_t raw_rows(int max_len) { return ((int64_t)max_len + 63) / 64 * 64; }
 
@@ -273,13 +274,16 @@ int tree_launch(const char *who, TreeParams &p, const void *workspace, size_t wo
         p.stats = (float *)(ws + record_bytes(p.B, p.n, p.Hq, p.Hkv, head_dim, max_total, cache_dtype));
         p.raw = (float *)((unsigned char *)p.stats + round256((size_t)p.B * p.Hq * 2 * sizeof(float)));
     }
-    p.chunk_rows = tree_chunk_rows(p.B, p.n, p.Hq, p.Hkv, max_total);
-    p.max_chunks = (int)(((int64_t)max_total + p.chunk_rows - 1) / p.chunk_rows);
-    const int q_tiles = (p.n * p.G + kBM - 1) / kBM;
-    const dim3 grid(p.max_chunks, p.Hkv * q_tiles, p.B);
-    cudaError_t e;
-    if (cache_dtype == NIMLLM_F32) e = head_dim == 64 ? launch_fma<float, 64>(p, grid, st) : launch_fma<float, 128>(p, grid, st);
-    else e = head_dim == 64 ? launch_fma<__nv_bfloat16, 64>(p, grid, st) : launch_fma<__nv_bfloat16, 128>(p, grid, st);
+    cudaError_t e = cudaSuccess;
+    if (use_tensor_cores(cache_dtype)) {
+        if (int rc = launch_tree_tc(who, p, head_dim, ws, st)) return rc;
+    } else {
+        p.chunk_rows = tree_chunk_rows(p.B, p.n, p.Hq, p.Hkv, max_total);
+        p.max_chunks = (int)(((int64_t)max_total + p.chunk_rows - 1) / p.chunk_rows);
+        const int q_tiles = (p.n * p.G + kBM - 1) / kBM;
+        const dim3 grid(p.max_chunks, p.Hkv * q_tiles, p.B);
+        e = head_dim == 64 ? launch_fma<float, 64>(p, grid, st) : launch_fma<float, 128>(p, grid, st);
+    }
     if (e == cudaSuccess && p.score) e = launch_dependent(tree_score_kernel, dim3((p.max_len + 255) / 256, p.Hkv, p.B), 256, 0, st, p);
     if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return NIMLLM_OK;

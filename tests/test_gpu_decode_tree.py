@@ -271,3 +271,7 @@ def test_scored_skips_rows_without_a_page(cache_dtype):
     got = score.cpu()[0].double()
     assert (got[:, 32:64] == 2.0).all()
     assert float((got - 2.0 - add).abs().max()) <= U.attention_tolerance(D, L, mag, 1.0, F) * float(add.max()) + 5 * 2.0 ** -24 * 3
+
+
+def test_zz_no_launch_gave_up():
+    assert A.decode_tree_status(reset=False) == 0
