@@ -240,7 +240,8 @@ size_t record_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, i
     return round256(use_tensor_cores(cache_dtype) ? tree_tc_workspace_bytes(batch, n, n_head, n_kv_head, head_dim)
                                                     : fma_record_bytes(batch, n, n_head, n_kv_head, head_dim, max_total));
 }
-int64_t raw_rows(int max_len) { return ((int64_t)max_len + 63) / 64 * 64; }
+// whole tiles of the tensor-core kernels are written
+int64_t raw_rows(int max_len) { return ((int64_t)max_len + 127) / 128 * 128; }
 
 template <typename T, int D>
 cudaError_t launch_fma(const TreeParams &p, dim3 grid, cudaStream_t st) {

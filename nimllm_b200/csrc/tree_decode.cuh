@@ -54,7 +54,6 @@ __device__ __forceinline__ int64_t tree_out_row(const TreeParams &p, int b, int 
 
 // the tensor-core kernel for bf16 caches (tree_decode_tc.cu)
 size_t tree_tc_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim);
-int tree_tc_status(int reset, int *status_out);
 int launch_tree_tc(const char *who, TreeParams &p, int head_dim, void *workspace, cudaStream_t st);
 
 }  // namespace nimllm

@@ -19,19 +19,15 @@
 // split: an fp32 q into three bf16 terms (2^-26 left), P into two terms for bf16 results (2^-17) and three for fp32 results.
 // The terms are further MMAs into the same accumulator.
 //
-// Work split: all tiles of the batch in one list ordered by (sequence, KV head, query tile, row), cut into equal spans, one per
-// CTA (one CTA per SM).  A CTA cuts at most two (sequence, KV head) pairs; their pieces go to its two record slots and
-// tree_tc_join_kernel finds them by the same arithmetic.
-//
 // Every wait is bounded as in prefill_tc.cu: after about 2 s without progress the CTA aborts and raises the status word.
-#include "tcgen05.cuh"
-#include "tree_decode.cuh"
+#include "tree_tc.cuh"
 
 namespace nimllm {
 
 namespace {
 
 using namespace tc;
+using namespace treetc;
 
 __device__ int g_tree_status = 0;      // sticky, nimllm_attn_decode_tree_status
 
@@ -43,93 +39,12 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColP = 64, kColO = 192;    // S | P terms (3 x 32) | O x 2
 constexpr int kQBox = kRows * 128, kKvBox = kTile * 128;  // bytes of a 64-column box
 
-struct TcArgs {
-    int64_t *cum;              // [B + 1] units before each sequence, written by CTA 0 for the join
-    int q_terms, p_terms, stages, lag;
-};
-
-__host__ __device__ inline int64_t first_unit(int w, int64_t T, int wa) { return (int64_t)w * T / wa; }
-__host__ __device__ inline int owner_of(int64_t u, int64_t T, int wa) { return (int)(((u + 1) * wa - 1) / T); }
-
-// what a sequence contributes: q tiles per KV head and tiles per q tile
-struct SeqWork {
-    int len, drafts, total, R, q_tiles, tiles;
-};
-template <int RPT> __device__ __forceinline__ SeqWork seq_work(const TreeParams &p, int b) {
-    SeqWork s;
-    s.len = tree_committed(p, b);
-    s.drafts = tree_drafts(p, b, s.len);
-    s.total = s.len + s.drafts;
-    s.R = tree_tokens(p, b) * p.G;
-    s.q_tiles = (s.R + RPT - 1) / RPT;
-    s.tiles = s.R ? (s.total + kTile - 1) / kTile : 0;
-    return s;
-}
-template <int RPT> __device__ __forceinline__ int64_t seq_units(const TreeParams &p, int b) {
-    const SeqWork s = seq_work<RPT>(p, b);
-    return (int64_t)p.Hkv * s.q_tiles * s.tiles;
-}
-
-// A CTA's span, segment by segment: tiles [i0, i1) of q tile qt of KV head kvh of sequence b
-struct Segment {
-    int b, kvh, qt, i0, i1;
-    SeqWork w;
-    bool whole;
-    int slot;
-};
-template <int RPT> struct SpanWalk {
-    const TreeParams &p;
-    int b, h, i0, remaining;
-    bool first;
-    SeqWork w;
-    __device__ SpanWalk(const TreeParams &p_, int b_, int h_, int i_, int n) : p(p_), b(b_), h(h_), i0(i_), remaining(n), first(true) {
-        if (n > 0) w = seq_work<RPT>(p, b);
-    }
-    __device__ bool next(Segment &s) {
-        if (remaining <= 0) return false;
-        while (w.tiles == 0 || h >= p.Hkv * w.q_tiles) {
-            b++; h = 0; i0 = 0;
-            w = seq_work<RPT>(p, b);
-        }
-        s.b = b; s.kvh = h / w.q_tiles; s.qt = h - s.kvh * w.q_tiles; s.w = w;
-        s.i0 = i0;
-        s.i1 = min(w.tiles, i0 + remaining);
-        s.whole = i0 == 0 && s.i1 == w.tiles;
-        s.slot = first ? 0 : 1;
-        remaining -= s.i1 - s.i0;
-        first = false;
-        i0 = s.i1;
-        if (i0 == w.tiles) { i0 = 0; h++; }
-        return true;
-    }
-};
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-// all but the newest n groups have landed (n <= 8)
-__device__ __forceinline__ void cp_wait(int n) {
-    switch (n) {
-        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-        case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-        case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-        case 7: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 8;" ::: "memory"); break;
-    }
-}
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t q_full, q_empty, s_full, s_free, p_ready, pv_done, epi, drain;
     uint32_t tmem_base;
     volatile int abort_flag;
-    int start_b, start_h, start_i;
-    int64_t warp_sum[kThreads / 32];
+    SpanStart start;
     int valid[kMaxStages];             // bit 0, 1: the pages of the tile's two halves exist
     float2 ml[kRows];                  // copies: maximum and sum of every lane, then of every row
 };
@@ -161,20 +76,6 @@ __device__ __forceinline__ uint64_t visible_rows(const TreeParams &p, const SeqW
     return vis;
 }
 
-template <int D>
-__device__ __forceinline__ void store_row4(const TreeParams &p, int64_t orow, int d, float4 x) {
-    if (p.out) {
-        if (p.out_dtype == NIMLLM_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.out) + orow * D + d) = x;
-        else *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + orow * D + d) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-    }
-    if (p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + d) = x;
-}
-template <int D>
-__device__ __forceinline__ void store_row_stats(const TreeParams &p, int64_t orow, float m, float l) {
-    if (p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + D) = make_float4(m * kLn2, l, 0.f, 0.f);
-    if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(m, l > 0.f ? 1.f / l : 0.f);
-}
-
 template <int D, int C>
 __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcArgs a) {
     constexpr int RPT = kRows / C;             // query rows of a tile
@@ -191,50 +92,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
     launch_dependents();
     grid_dependency_wait();
 
-    // ---- this CTA's span: prefix of the sequences' units over the block
-    const int per = (p.B + kThreads - 1) / kThreads;
-    const int b_beg = min(p.B, (int)threadIdx.x * per), b_end = min(p.B, b_beg + per);
-    int64_t sum = 0;
-    for (int b = b_beg; b < b_end; b++) sum += seq_units<RPT>(p, b);
-    int64_t incl = sum;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += x;
-    }
-    if (lane == 31) sb.warp_sum[warp] = incl;
-    if (threadIdx.x == 0) sb.abort_flag = 0;
-    __syncthreads();
-    int64_t excl = incl - sum, T = 0;
-    for (int w = 0; w < kThreads / 32; w++) {
-        if (w < warp) excl += sb.warp_sum[w];
-        T += sb.warp_sum[w];
-    }
-    if (blockIdx.x == 0) {
-        int64_t c = excl;
-        for (int b = b_beg; b < b_end; b++) { a.cum[b] = c; c += seq_units<RPT>(p, b); }
-        if (threadIdx.x == 0) a.cum[p.B] = T;
-    }
-    const int wa = (int)(T < (int64_t)gridDim.x ? T : (int64_t)gridDim.x);
-    if ((int)blockIdx.x >= wa) return;
-    const int64_t u0 = first_unit(blockIdx.x, T, wa);
-    const int n_units = (int)(first_unit(blockIdx.x + 1, T, wa) - u0);
-    if (u0 >= excl && u0 < excl + sum) {
-        int64_t c = excl;
-        for (int b = b_beg; b < b_end; b++) {
-            const SeqWork w = seq_work<RPT>(p, b);
-            const int64_t n = (int64_t)p.Hkv * w.q_tiles * w.tiles;
-            if (u0 < c + n) {
-                sb.start_b = b;
-                sb.start_h = (int)((u0 - c) / w.tiles);
-                sb.start_i = (int)((u0 - c) % w.tiles);
-                break;
-            }
-            c += n;
-        }
-    }
+    const int n_units = span_begin<RPT, kTile, kThreads>(p, a, sb.start);
+    if (n_units == 0) return;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < a.stages; s++) { mbar_init(&sb.full[s], 64); mbar_init(&sb.empty[s], 1); }
+        sb.abort_flag = 0;
+        for (int s = 0; s < a.stages; s++) { mbar_init(&sb.full[s], 65); mbar_init(&sb.empty[s], 1); }
         mbar_init(&sb.q_full, 32); mbar_init(&sb.q_empty, 1);
         mbar_init(&sb.s_full, 1); mbar_init(&sb.s_free, 4);
         mbar_init(&sb.p_ready, 4); mbar_init(&sb.pv_done, 1);
@@ -253,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
     tc_fence_after();
     const uint32_t tmem = sb.tmem_base;
     volatile int *abort_flag = &sb.abort_flag;
-    SpanWalk<RPT> walk(p, sb.start_b, sb.start_h, sb.start_i, n_units);
+    SpanWalk<RPT, kTile> walk(p, sb.start.b, sb.start.h, sb.start.i, n_units);
     Segment sg;
     bool ok = true;
 
@@ -266,7 +128,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
         const uint32_t kv = smem_u32(s_kv);
         const __nv_bfloat16 *kg = reinterpret_cast<const __nv_bfloat16 *>(p.k) + c * 8, *vg = reinterpret_cast<const __nv_bfloat16 *>(p.v) + c * 8;
         int k = 0;                                         // tiles issued
-        auto publish = [&](int tile) { fence_async(); mbar_arrive(&sb.full[tile % a.stages]); };
         while (ok && walk.next(sg)) {
             for (int i = sg.i0; ok && i < sg.i1; i++, k++) {
                 const int slot = k % a.stages, t0 = i * kTile;
@@ -275,7 +136,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
                 const int64_t h0 = cache_row(p.rows, sg.b, sg.kvh, t0);
                 const int64_t h1 = n > 32 ? cache_row(p.rows, sg.b, sg.kvh, t0 + 32) : 0;
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(&sb.empty[slot], ((k / a.stages) & 1) ^ 1, abort_flag)))) break;
-                if (t == 0) sb.valid[slot] = (h0 >= 0 ? 1 : 0) | (h1 >= 0 ? 2 : 0);
+                if (t == 0) {                              // the 65th arrival publishes the word
+                    sb.valid[slot] = (h0 >= 0 ? 1 : 0) | (h1 >= 0 ? 2 : 0);
+                    mbar_arrive(&sb.full[slot]);
+                }
                 const uint32_t dst = kv + slot * kStage + (c >> 3) * kKvBox;
 #pragma unroll
                 for (int r0 = 0; r0 < kTile; r0 += kStep) {
@@ -287,16 +151,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
                     cp_async16(d, kg + off, have ? 16 : 0);
                     cp_async16(d + kKv, vg + off, have ? 16 : 0);
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (k >= a.lag) {
-                    cp_wait(a.lag);
-                    publish(k - a.lag);
-                }
+                cp_async_arrive(&sb.full[slot]);
             }
         }
-        cp_wait(0);
-        if (ok)
-            for (int x = max(0, k - a.lag); x < k; x++) publish(x);
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 6) {
         // ---------------------------------------------------------------- Q
         const uint32_t qs = smem_u32(s_q);
@@ -373,6 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
         auto issue_s = [&](int tile) -> bool {
             if (!mbar_wait(&sb.full[tile % a.stages], (tile / a.stages) & 1, abort_flag)) return false;
             if (tile > 0 && !mbar_wait(&sb.s_free, (tile - 1) & 1, abort_flag)) return false;
+            fence_async();
             tc_fence_after();
             const uint32_t k_lo = (((kv_base + (uint32_t)(tile % a.stages) * kStage) >> 4) & 0x3FFFu) | kLboK;
             for (int t = 0; t < a.q_terms; t++)
@@ -539,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
             tc_fence_before();
 
             constexpr int W = D + 4;
-            float *rec = sg.whole ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + sg.slot) * kRows * W;
+            float *rec = sg.whole ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + sg.slot) * kRecRows * W;
             if constexpr (C == 1) {
                 if (live) {
                     const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -603,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
 
 // One warp per row of out: the pieces of a cut (sequence, KV head, query tile); zeros where a token has no row at all.
 template <int D>
-__global__ void __launch_bounds__(128) tree_tc_join_kernel(TreeParams p, TcArgs a, int RPT, int workers) {
+__global__ void __launch_bounds__(128) tree_tc_join_kernel(TreeParams p, TcArgs a, int RPT, int TILE, int workers) {
     launch_dependents();
     grid_dependency_wait();
     const int64_t orow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -621,13 +480,13 @@ __global__ void __launch_bounds__(128) tree_tc_join_kernel(TreeParams p, TcArgs 
     }
     const int64_t T = a.cum[p.B];
     const int wa = (int)(T < workers ? T : workers);
-    const int q_tiles = (tokens * p.G + RPT - 1) / RPT, tiles = (total + kTile - 1) / kTile;
+    const int q_tiles = (tokens * p.G + RPT - 1) / RPT, tiles = (total + TILE - 1) / TILE;
     const int kvh = hq / p.G, qr = i * p.G + hq % p.G, qt = qr / RPT, r = qr % RPT;
     const int64_t s = a.cum[b] + ((int64_t)kvh * q_tiles + qt) * tiles;
     const int w0 = owner_of(s, T, wa), n = owner_of(s + tiles - 1, T, wa) - w0 + 1;
     if (n == 1) return;
     const int slot0 = first_unit(w0, T, wa) < s ? 1 : 0;
-    auto rec_of = [&](int x) { return p.recs + (((int64_t)(w0 + x) * 2 + (x == 0 ? slot0 : 0)) * kRows + r) * W; };
+    auto rec_of = [&](int x) { return p.recs + (((int64_t)(w0 + x) * 2 + (x == 0 ? slot0 : 0)) * kRecRows + r) * W; };
     float M = -INFINITY;
     for (int x = lane; x < n; x += 32) {
         const float *rec = rec_of(x);
@@ -657,9 +516,7 @@ __global__ void __launch_bounds__(128) tree_tc_join_kernel(TreeParams p, TcArgs 
     if (lane == 0) store_row_stats<D>(p, orow, M * kLog2e, sum);
 }
 
-size_t rec_bytes(int head_dim) { return (size_t)sm_count() * 2 * kRows * rec_stride(head_dim) * sizeof(float); }
-
-constexpr size_t kSmemMost = 227 * 1024 - sizeof(Bars) - 1024;     // dynamic: what is left beside Bars and the alignment
+constexpr size_t kSmemMost = 227 * 1024 - (sizeof(Bars) + 1023) / 1024 * 1024 - 1024;     // dynamic: beside Bars, and 1024 bytes to align
 
 template <int D, int C>
 cudaError_t launch_c(const TreeParams &p, TcArgs &a, cudaStream_t st) {
@@ -670,7 +527,6 @@ cudaError_t launch_c(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     const size_t q = (size_t)a.q_terms * kRows * D * 2, stage = 2 * kTile * D * 2, join = C > 1 ? kRows * 33 * sizeof(float) : 0;
     int stages = (int)((kSmemMost - q - join) / stage);
     a.stages = stages > kMaxStages ? kMaxStages : stages;
-    a.lag = a.stages - 2;              // the ring never waits for a tile that it has not published
     if (dev >= 64 || !ready[dev]) {
         e = cudaFuncSetAttribute(tree_tc_kernel<D, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMost + 1024));
         if (e != cudaSuccess) return e;
@@ -682,10 +538,14 @@ cudaError_t launch_c(const TreeParams &p, TcArgs &a, cudaStream_t st) {
 template <int D>
 cudaError_t launch_d(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     const int R = p.n * p.G;
-    cudaError_t e = R <= 32 ? launch_c<D, 4>(p, a, st) : (R <= 64 ? launch_c<D, 2>(p, a, st) : launch_c<D, 1>(p, a, st));
+    const bool narrow = tree_narrow_takes(R, a.q_terms, a.p_terms, D);
+    const int rpt = narrow ? kNarrowRows : (R <= 32 ? 32 : (R <= 64 ? 64 : 128));
+    cudaError_t e;
+    if (narrow) e = launch_tree_narrow(p, a, D, st);
+    else e = rpt == 32 ? launch_c<D, 4>(p, a, st) : (rpt == 64 ? launch_c<D, 2>(p, a, st) : launch_c<D, 1>(p, a, st));
     if (e != cudaSuccess) return e;
     const int64_t rows = (int64_t)p.B * p.n * p.Hq;
-    return launch_dependent(tree_tc_join_kernel<D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, p, a, R <= 32 ? 32 : (R <= 64 ? 64 : 128), sm_count());
+    return launch_dependent(tree_tc_join_kernel<D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, p, a, rpt, narrow ? kNarrowTile : kTile, sm_count());
 }
 
 }  // namespace
@@ -701,27 +561,30 @@ int launch_tree_tc(const char *who, TreeParams &p, int head_dim, void *workspace
     a.cum = (int64_t *)((unsigned char *)workspace + rec_bytes(head_dim));
     a.q_terms = p.q_dtype == NIMLLM_F32 ? 3 : 1;
     a.p_terms = (p.out && p.out_dtype == NIMLLM_F32) || p.partials_out ? 3 : 2;
+    a.stages = 0;
     const cudaError_t e = head_dim == 64 ? launch_d<64>(p, a, st) : launch_d<128>(p, a, st);
     if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return NIMLLM_OK;
 }
 
-int tree_tc_status(int reset, int *status_out) {
+// Reads (and clears) a sticky word of the current device.
+template <typename T> static int read_status(T &word, int reset, int *out) {
     int st = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&st, g_tree_status, sizeof(int));
+    cudaError_t e = cudaMemcpyFromSymbol(&st, word, sizeof(int));
     if (e == cudaSuccess && reset && st != 0) {
         const int zero = 0;
-        e = cudaMemcpyToSymbol(g_tree_status, &zero, sizeof(int));
+        e = cudaMemcpyToSymbol(word, &zero, sizeof(int));
     }
     if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "attn_decode_tree_status: %s", cudaGetErrorString(e));
-    *status_out = st;
+    *out = st;
     return NIMLLM_OK;
 }
 
 }  // namespace nimllm
 
 extern "C" int nimllm_attn_decode_tree_status(int reset) {
-    int st = 0;
-    const int rc = nimllm::tree_tc_status(reset, &st);
-    return rc ? -rc : st;
+    int wide = 0, narrow = 0;
+    int rc = nimllm::read_status(nimllm::g_tree_status, reset, &wide);
+    if (!rc) rc = nimllm::treetc::tree_narrow_status(reset, &narrow);
+    return rc ? -rc : (wide | narrow);
 }
