@@ -5,7 +5,7 @@
 //
 // This file holds the entry points, the CUDA-core kernel and the launches that finish a call.  The G query heads of a KV head
 // and the n tokens of a sequence are rows of one tile, so that a cached row is read once for all of them.
-#include "tree_decode.cuh"
+#include "tree_finish.cuh"
 
 namespace nimllm {
 
@@ -159,69 +159,6 @@ __global__ void __launch_bounds__(256) tree_fma_kernel(TreeParams p) {
     }
 }
 
-// One warp per row of out: the chunks of its sequence joined by their maxima and sums.
-template <int D>
-__global__ void __launch_bounds__(128) tree_join_kernel(TreeParams p) {
-    launch_dependents();
-    grid_dependency_wait();
-    const int64_t orow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (orow >= (int64_t)p.B * p.n * p.Hq) return;
-    const int b = (int)(orow / ((int64_t)p.n * p.Hq)), i = (int)(orow / p.Hq % p.n);
-    if (i >= tree_tokens(p, b)) return;
-    const int len = tree_committed(p, b), total = len + tree_drafts(p, b, len);
-    const int n = (total + p.chunk_rows - 1) / p.chunk_rows;
-    if (n <= 1) return;
-    constexpr int W = D + 4;
-    const int64_t step = (int64_t)p.B * p.n * p.Hq * W;
-    const float *rec = p.recs + orow * W;
-    float M = -INFINITY;
-    for (int c = lane; c < n; c += 32)
-        if (rec[c * step + D + 1] > 0.f) M = fmaxf(M, rec[c * step + D]);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    const float safe = M == -INFINITY ? 0.f : M;
-    float acc[D / 32], sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 32; j++) acc[j] = 0.f;
-    for (int c = 0; c < n; c++) {
-        const float *r = rec + c * step;
-        const float lc = r[D + 1], w = lc > 0.f ? lc * ex2((r[D] - safe) * kLog2e) : 0.f;
-        sum += w;
-#pragma unroll
-        for (int j = 0; j < D / 32; j++) acc[j] = fmaf(w, r[lane + 32 * j], acc[j]);
-    }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 32; j++) {
-        const int d = lane + 32 * j;
-        if (p.out) store_from_f32(p.out, p.out_dtype, orow * D + d, acc[j] * inv);
-        if (p.partials_out) p.partials_out[orow * W + d] = acc[j] * inv;
-    }
-    if (lane == 0) {
-        if (p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * W + D) = make_float4(M, sum, 0.f, 0.f);
-        if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(M * kLog2e, inv);
-    }
-}
-
-// score[r] = decay * score[r] + sum over the G heads of exp2(raw - m) / l.  A row without a page has no raw score.
-__global__ void __launch_bounds__(256) tree_score_kernel(TreeParams p) {
-    launch_dependents();
-    grid_dependency_wait();
-    const int kvh = blockIdx.y, b = blockIdx.z;
-    const int len = tree_committed(p, b);
-    const int r = blockIdx.x * 256 + threadIdx.x;
-    if (r >= len || (p.rows.table && cache_row(p.rows, b, kvh, r) < 0)) return;
-    float sum = 0.f;
-    for (int g = 0; g < p.G; g++) {
-        const int64_t h = (int64_t)b * p.Hq + kvh * p.G + g;
-        const float2 st = *reinterpret_cast<const float2 *>(p.stats + 2 * h);
-        sum += ex2(p.raw[h * p.raw_ld + r] - st.x) * st.y;
-    }
-    float *s = p.score + ((int64_t)b * p.Hkv + kvh) * p.score_rows + r;
-    *s = (p.decay == 0.f ? 0.f : p.decay * *s) + sum;
-}
-
 // rows of a chunk: enough CTAs for four on every SM, at least 128 rows each
 int tree_chunk_rows(int batch, int n, int n_head, int n_kv_head, int max_total) {
     const int64_t tiles = (int64_t)batch * n_kv_head * (((int64_t)n * (n_head / n_kv_head) + kBM - 1) / kBM);
@@ -255,9 +192,8 @@ cudaError_t launch_fma(const TreeParams &p, dim3 grid, cudaStream_t st) {
         if (dev < 64) ready[dev] = true;
     }
     e = launch_dependent(tree_fma_kernel<T, D>, grid, 256, fma_smem<D>(), st, p);
-    const int64_t rows = (int64_t)p.B * p.n * p.Hq;
-    if (e == cudaSuccess && p.max_chunks > 1) e = launch_dependent(tree_join_kernel<D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, p);
-    return e;
+    treetc::FinishArgs f = {};
+    return e == cudaSuccess ? treetc::launch_finish<D>(p, f, st) : e;
 }
 
 // q, shapes and the workspace of both entry points
@@ -285,7 +221,6 @@ int tree_launch(const char *who, TreeParams &p, const void *workspace, size_t wo
         const dim3 grid(p.max_chunks, p.Hkv * q_tiles, p.B);
         e = head_dim == 64 ? launch_fma<float, 64>(p, grid, st) : launch_fma<float, 128>(p, grid, st);
     }
-    if (e == cudaSuccess && p.score) e = launch_dependent(tree_score_kernel, dim3((p.max_len + 255) / 256, p.Hkv, p.B), 256, 0, st, p);
     if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return NIMLLM_OK;
 }

@@ -20,7 +20,7 @@
 // The terms are further MMAs into the same accumulator.
 //
 // Every wait is bounded as in prefill_tc.cu: after about 2 s without progress the CTA aborts and raises the status word.
-#include "tree_tc.cuh"
+#include "tree_finish.cuh"
 
 namespace nimllm {
 
@@ -460,62 +460,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(TreeParams p, TcAr
     }
 }
 
-// One warp per row of out: the pieces of a cut (sequence, KV head, query tile); zeros where a token has no row at all.
-template <int D>
-__global__ void __launch_bounds__(128) tree_tc_join_kernel(TreeParams p, TcArgs a, int RPT, int TILE, int workers) {
-    launch_dependents();
-    grid_dependency_wait();
-    const int64_t orow = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (orow >= (int64_t)p.B * p.n * p.Hq) return;
-    const int b = (int)(orow / ((int64_t)p.n * p.Hq)), i = (int)(orow / p.Hq % p.n), hq = (int)(orow % p.Hq);
-    const int tokens = tree_tokens(p, b);
-    if (i >= tokens) return;
-    constexpr int W = D + 4;
-    const int len = tree_committed(p, b), total = len + tree_drafts(p, b, len);
-    if (total == 0) {
-        for (int d = lane * 4; d < D; d += 128) store_row4<D>(p, orow, d, make_float4(0.f, 0.f, 0.f, 0.f));
-        if (lane == 0) store_row_stats<D>(p, orow, -INFINITY, 0.f);
-        return;
-    }
-    const int64_t T = a.cum[p.B];
-    const int wa = (int)(T < workers ? T : workers);
-    const int q_tiles = (tokens * p.G + RPT - 1) / RPT, tiles = (total + TILE - 1) / TILE;
-    const int kvh = hq / p.G, qr = i * p.G + hq % p.G, qt = qr / RPT, r = qr % RPT;
-    const int64_t s = a.cum[b] + ((int64_t)kvh * q_tiles + qt) * tiles;
-    const int w0 = owner_of(s, T, wa), n = owner_of(s + tiles - 1, T, wa) - w0 + 1;
-    if (n == 1) return;
-    const int slot0 = first_unit(w0, T, wa) < s ? 1 : 0;
-    auto rec_of = [&](int x) { return p.recs + (((int64_t)(w0 + x) * 2 + (x == 0 ? slot0 : 0)) * kRecRows + r) * W; };
-    float M = -INFINITY;
-    for (int x = lane; x < n; x += 32) {
-        const float *rec = rec_of(x);
-        if (rec[D + 1] > 0.f) M = fmaxf(M, rec[D]);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    const float safe = M == -INFINITY ? 0.f : M;
-    float acc[D / 32], sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 32; j++) acc[j] = 0.f;
-#pragma unroll 4
-    for (int x = 0; x < n; x++) {
-        const float *rec = rec_of(x);
-        const float lc = rec[D + 1], w = lc > 0.f ? lc * ex2((rec[D] - safe) * kLog2e) : 0.f;
-        sum += w;
-#pragma unroll
-        for (int j = 0; j < D / 32; j++) acc[j] = fmaf(w, rec[lane + 32 * j], acc[j]);
-    }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 32; j++) {
-        const int d = lane + 32 * j;
-        if (p.out) store_from_f32(p.out, p.out_dtype, orow * D + d, acc[j] * inv);
-        if (p.partials_out) p.partials_out[orow * W + d] = acc[j] * inv;
-    }
-    if (lane == 0) store_row_stats<D>(p, orow, M * kLog2e, sum);
-}
-
 constexpr size_t kSmemMost = 227 * 1024 - (sizeof(Bars) + 1023) / 1024 * 1024 - 1024;     // dynamic: beside Bars, and 1024 bytes to align
 
 template <int D, int C>
@@ -544,21 +488,23 @@ cudaError_t launch_d(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     if (narrow) e = launch_tree_narrow(p, a, D, st);
     else e = rpt == 32 ? launch_c<D, 4>(p, a, st) : (rpt == 64 ? launch_c<D, 2>(p, a, st) : launch_c<D, 1>(p, a, st));
     if (e != cudaSuccess) return e;
-    const int64_t rows = (int64_t)p.B * p.n * p.Hq;
-    return launch_dependent(tree_tc_join_kernel<D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, p, a, rpt, narrow ? kNarrowTile : kTile, sm_count());
+    FinishArgs f = {};
+    f.tc = a; f.rpt = rpt; f.tile = narrow ? kNarrowTile : kTile; f.workers = sm_count();
+    return launch_finish<D>(p, f, st);
 }
 
 }  // namespace
 
 size_t tree_tc_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim) {
     (void)n; (void)n_head; (void)n_kv_head;
-    return rec_bytes(head_dim) + ((size_t)batch + 1) * sizeof(int64_t);
+    return rec_bytes(head_dim) + (size_t)sm_count() * sizeof(int4) + ((size_t)batch + 1) * sizeof(int64_t);
 }
 
 int launch_tree_tc(const char *who, TreeParams &p, int head_dim, void *workspace, cudaStream_t st) {
-    TcArgs a;
+    TcArgs a = {};
     p.recs = (float *)workspace;
-    a.cum = (int64_t *)((unsigned char *)workspace + rec_bytes(head_dim));
+    a.starts = (int4 *)((unsigned char *)workspace + rec_bytes(head_dim));
+    a.cum = (int64_t *)(a.starts + sm_count());
     a.q_terms = p.q_dtype == NIMLLM_F32 ? 3 : 1;
     a.p_terms = (p.out && p.out_dtype == NIMLLM_F32) || p.partials_out ? 3 : 2;
     a.stages = 0;

@@ -9,9 +9,10 @@
 //   warps 0-3, 4-7   two softmax groups, taking the tiles of 128 rows in turn: the waits of one hide behind the other
 //   warps 8-11       K rows (8, 9) and V rows (10, 11) into a ring of slots with cp.async, swizzled, exact to the row
 //                    (tree_decode_tc.cu says why no TMA)
-//   warp 12          Q of the segments to come (two buffers), and which query rows see each of their drafts
+//   warp 12          walks the CTA's span and hands its segments to the others; Q of the segments to come (two buffers), and which
+//                    query rows see each of their drafts
 //   warps 13, 14     issue K Q^T and V^T P^T, each in order and waiting for its own operands alone
-//   warp 15          walks the CTA's span and hands the segments to the others
+//   warp 15          joins the two groups' sums at the end of a segment and stores them, beside the next one's tiles
 //
 // Softmax across threads: with one thread per cached row a query row's maximum lies across 128 threads.  It is not needed: a
 // reference per query row that some score has and none passes by more than 2^32 serves as well, because P is rounded relative to
@@ -89,37 +90,19 @@ template <int N> __device__ __forceinline__ void tmem_st(uint32_t at, const uint
     else if constexpr (N == 8) tmem_st8(at, r);
     else asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
-// x = (ADD: x +) the sum of the terms' columns of an accumulator.  All loads are in flight together where registers allow: for few
-// columns, and for 16 of S, when x is not alive yet.
-template <int N, int RP, bool ADD> __device__ __forceinline__ void tmem_terms(uint32_t at, int terms, float *x) {
-    if constexpr (N <= 8 || (N == 16 && !ADD)) {
-        uint32_t y[N], z[N], v[N];
-        tmem_ld<N>(at, y);
-        if (terms > 1) tmem_ld<N>(at + RP, z);
-        if (terms > 2) tmem_ld<N>(at + 2 * RP, v);
+// x = (ADD: x +) the sum of the TERMS' columns of an accumulator, all loads in flight together where registers allow
+template <int N, int RP, int TERMS, bool ADD> __device__ __forceinline__ void tmem_terms(uint32_t at, float *x) {
+    constexpr int kBatch = N <= 16 ? TERMS : 1;
+#pragma unroll
+    for (int t0 = 0; t0 < TERMS; t0 += kBatch) {
+        uint32_t y[kBatch][N];
+#pragma unroll
+        for (int t = 0; t < kBatch; t++) tmem_ld<N>(at + (t0 + t) * RP, y[t]);
         tc_wait_ld();
 #pragma unroll
-        for (int r = 0; r < N; r++) x[r] = ADD ? x[r] + __uint_as_float(y[r]) : __uint_as_float(y[r]);
-        if (terms > 1) {
+        for (int r = 0; r < N; r++)
 #pragma unroll
-            for (int r = 0; r < N; r++) x[r] += __uint_as_float(z[r]);
-        }
-        if (terms > 2) {
-#pragma unroll
-            for (int r = 0; r < N; r++) x[r] += __uint_as_float(v[r]);
-        }
-    } else {
-        uint32_t y[N];
-        tmem_ld<N>(at, y);
-        tc_wait_ld();
-#pragma unroll
-        for (int r = 0; r < N; r++) x[r] = ADD ? x[r] + __uint_as_float(y[r]) : __uint_as_float(y[r]);
-        for (int t = 1; t < terms; t++) {
-            tmem_ld<N>(at + t * RP, y);
-            tc_wait_ld();
-#pragma unroll
-            for (int r = 0; r < N; r++) x[r] += __uint_as_float(y[r]);
-        }
+            for (int t = 0; t < kBatch; t++) x[r] = ADD || t0 + t > 0 ? x[r] + __uint_as_float(y[t][r]) : __uint_as_float(y[t][r]);
     }
 }
 
@@ -151,16 +134,16 @@ __device__ __forceinline__ bool next_segment(Bars &sb, int s, SegEntry &e, bool 
     return e.b >= 0;
 }
 
-// RC: query rows that are computed (the rest of the 16 or 32 columns stays zero)
-template <int D, int RC>
+// RC: query rows that are computed (the rest of the 16 or 32 columns stays zero); NQ, NP: terms of q and of P
+template <int D, int RC, int NQ, int NP>
 __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, TcArgs a) {
     constexpr int RP = RC <= 16 ? 16 : 32;     // columns of a term
     constexpr int kSlot = kTile * D * 2;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Bars sb;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const int n_s = RP * a.q_terms, n_o = RP * a.p_terms;
-    const int q_box = n_s * 128, q_bytes = n_s * D * 2;
+    constexpr int n_s = RP * NQ, n_o = RP * NP;
+    constexpr int q_box = n_s * 128, q_bytes = n_s * D * 2;
     uint8_t *s_kv = smem, *s_p = s_kv + a.stages * kSlot, *s_q = s_p + 2 * kPBytes;
     float *s_x = reinterpret_cast<float *>(s_q + 2 * q_bytes);       // the groups' O at the end of a segment: [2][RC][D]
 
@@ -178,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
             mbar_init(&sb.s_full[g], 1); mbar_init(&sb.s_free[g], 4);
             mbar_init(&sb.p_ready[g], 4); mbar_init(&sb.pv_done[g], 1);
         }
-        mbar_init(&sb.q_asked, 32); mbar_init(&sb.x_ready, 4); mbar_init(&sb.x_free, 4); mbar_init(&sb.drain[0], 1); mbar_init(&sb.drain[1], 1);
+        mbar_init(&sb.q_asked, 32); mbar_init(&sb.x_ready, 8); mbar_init(&sb.x_free, 1); mbar_init(&sb.drain[0], 1); mbar_init(&sb.drain[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // columns that no query row fills stay zero, in Q and in P
@@ -244,7 +227,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
     } else if (warp == 12) {
         // ---------------------------------------------------------------- Q: row r of term t is row t * RP + r of the B operand
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        for (int seg = 0; next_segment(sb, seg, sg, ok, lane); seg++) {
+        SpanWalk<kNarrowRows, kTile> walk(p, sb.start.b, sb.start.h, sb.start.i, n_units);
+        for (int seg = 0;; seg++) {
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&sb.seg_empty[seg % kSegs], ((seg / kSegs) & 1) ^ 1, abort_flag)))) break;
+            Segment s;
+            const bool more = walk.next(s);
+            sg = more ? SegEntry{s.b, s.kvh, s.i0, s.i1, s.w.len, s.w.total, s.w.R, (s.whole ? 1 : 0) | (s.slot ? 2 : 0)} : SegEntry{-1, 0, 0, 0, 0, 0, 0, 0};
+            if (lane == 0) {
+                sb.segs[seg % kSegs] = sg;
+                mbar_arrive(&sb.seg_full[seg % kSegs]);
+            }
+            if (!more) break;
             const int buf = seg & 1;
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(&sb.q_empty[buf], ((seg >> 1) & 1) ^ 1, abort_flag)))) break;
             const uint32_t qs = smem_u32(s_q) + buf * q_bytes;
@@ -255,8 +248,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                 const int token = lane / p.G;
                 bits = p.mask ? p.mask[((int64_t)sg.b * p.n + token) * p.words] : (2ull << token) - 1;
             }
-            const bool f32 = p.q_dtype == NIMLLM_F32;
-            const int chunks = f32 ? D / 4 : D / 8, step = 32 / chunks, c = lane % chunks;      // 16-byte pieces of a row of q
+            constexpr bool f32 = NQ == 3;
+            constexpr int chunks = f32 ? D / 4 : D / 8, step = 32 / chunks;      // 16-byte pieces of a row of q
+            const int c = lane % chunks;
             const char *qg = reinterpret_cast<const char *>(p.q) + c * 16;
             for (int r0 = 0; r0 < rows; r0 += 8 * step) {
                 uint4 x[8];
@@ -362,18 +356,38 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
         tc_commit_if(leader, &sb.drain[1]);
         mbar_wait(&sb.drain[1], 0, abort_flag);
     } else if (warp == 15) {
-        // ---------------------------------------------------------------- the CTA's segments
+        // ---------------------------------------------------------------- results
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        SpanWalk<kNarrowRows, kTile> walk(p, sb.start.b, sb.start.h, sb.start.i, n_units);
-        Segment s;
-        for (int seg = 0, more = 1; more; seg++) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sb.seg_empty[seg % kSegs], ((seg / kSegs) & 1) ^ 1, abort_flag))) break;
-            more = walk.next(s);
-            if (lane == 0) {
-                sb.segs[seg % kSegs] = more ? SegEntry{s.b, s.kvh, s.i0, s.i1, s.w.len, s.w.total, s.w.R, (s.whole ? 1 : 0) | (s.slot ? 2 : 0)}
-                                            : SegEntry{-1, 0, 0, 0, 0, 0, 0, 0};
-                mbar_arrive(&sb.seg_full[seg % kSegs]);
+        constexpr int W = D + 4;
+        for (int seg = 0; next_segment(sb, seg, sg, ok, lane); seg++) {
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&sb.x_ready, seg & 1, abort_flag)))) break;
+            float *rec = sg.flags & 1 ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * kRecRows * W;
+            if (lane < sg.R) {                             // lane r: how much of each group's O counts
+                const int r = lane;
+                const float r0 = sb.xref[0][r], r1 = sb.xref[1][r];
+                const float s0 = (sb.wsum[0][0][r] + sb.wsum[0][1][r]) + (sb.wsum[0][2][r] + sb.wsum[0][3][r]);
+                const float s1 = (sb.wsum[1][0][r] + sb.wsum[1][1][r]) + (sb.wsum[1][2][r] + sb.wsum[1][3][r]);
+                const float M = fmaxf(r0, r1), m = M == kUnset ? -INFINITY : M;
+                const float f0 = ex2(r0 - M), f1 = ex2(r1 - M);
+                const float L = s0 * f0 + s1 * f1, inv = L > 0.f ? 1.f / L : 0.f;
+                const int64_t orow = tree_out_row(p, sg.b, sg.kvh, r);
+                sb.join[r] = make_float2(f0 * inv, f1 * inv);
+                sb.orow[r] = orow;
+                if (rec) *reinterpret_cast<float4 *>(rec + r * W + D) = make_float4(m * kLn2, L, 0.f, 0.f);
+                else store_row_stats<D>(p, orow, m, L);
             }
+            __syncwarp();
+#pragma unroll 2
+            for (int e = lane; e < sg.R * (D / 4); e += 32) {
+                const int r = e / (D / 4), col = e % (D / 4) * 4;
+                const float2 f = sb.join[r];
+                const float4 o0 = *reinterpret_cast<const float4 *>(s_x + r * D + col), o1 = *reinterpret_cast<const float4 *>(s_x + (RC + r) * D + col);
+                const float4 v = make_float4(o0.x * f.x + o1.x * f.y, o0.y * f.x + o1.y * f.y, o0.z * f.x + o1.z * f.y, o0.w * f.x + o1.w * f.y);
+                if (rec) *reinterpret_cast<float4 *>(rec + r * W + col) = v;
+                else store_row4<D>(p, sb.orow[r], col, v);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sb.x_free);
         }
     } else {
         // ---------------------------------------------------------------- softmax groups
@@ -406,12 +420,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                 float x[RC];
                 bool grown = !ok;
                 if (ok) {
-                    tmem_terms<RC, RP, false>(s_at, a.q_terms, x);
+                    tmem_terms<RC, RP, NQ, false>(s_at, x);
                     const int valid = sb.valid[kk & 7];
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sb.s_free[g]);
-                    if (jg > 0 && jg % kWindow == 0) tmem_terms<RC, RP, true>(o_at, a.p_terms, acc);
+                    if (jg > 0 && jg % kWindow == 0) tmem_terms<RC, RP, NP, true>(o_at, acc);
 #pragma unroll
                     for (int r = 0; r < RC; r++) x[r] *= c;
                     const int at = t0 + row;
@@ -438,10 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                     }
                     group_any(g, false);
                 }
+                float ref[RC];
+#pragma unroll
+                for (int r = 0; r < RC; r++) ref[r] = sb.ref[g][r];
                 if (ok) {
                     float top = -INFINITY;
 #pragma unroll
-                    for (int r = 0; r < RC; r++) top = fmaxf(top, x[r] - sb.ref[g][r]);
+                    for (int r = 0; r < RC; r++) top = fmaxf(top, x[r] - ref[r]);
                     grown = top > kGrow;
                 }
                 if (group_any(g, grown)) {
@@ -458,14 +475,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                     float f[RC];
 #pragma unroll
                     for (int r = 0; r < RC; r++) {
-                        const float old = sb.ref[g][r];
                         const float m = fmaxf(fmaxf(sb.wmax[g][0][r], sb.wmax[g][1][r]), fmaxf(sb.wmax[g][2][r], sb.wmax[g][3][r]));
-                        f[r] = m > old + kGrow && m < INFINITY ? ex2(old - m) : 1.f;
+                        f[r] = 1.f;
+                        if (m > ref[r] + kGrow && m < INFINITY) {
+                            f[r] = ex2(ref[r] - m);
+                            ref[r] = m;
+                        }
+                        if (row == 0) sb.ref[g][r] = ref[r];
                         l[r] *= f[r];
                         acc[r] *= f[r];
                     }
                     if (jg % kWindow != 0) {
-                        for (int t = 0; t < a.p_terms; t++) {
+#pragma unroll
+                        for (int t = 0; t < NP; t++) {
                             uint32_t o[RC];
                             tmem_ld<RC>(o_at + t * RP, o);
                             tc_wait_ld();
@@ -475,37 +497,40 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                         }
                         tc_wait_st();
                     }
-                    group_any(g, false);
-                    if (row < RC) {
-                        const float m = fmaxf(fmaxf(sb.wmax[g][0][row], sb.wmax[g][1][row]), fmaxf(sb.wmax[g][2][row], sb.wmax[g][3][row]));
-                        if (m > sb.ref[g][row] + kGrow && m < INFINITY) sb.ref[g][row] = m;
-                    }
-                    group_any(g, false);
+                    group_any(g, false);                                       // wmax is read, ref written
                 }
-                // P^T in two or three bf16 terms, eight columns (RC = 4: four) at a time
-                constexpr int kGroup = RC < 8 ? RC : 8;
+                // P^T in two or three bf16 terms, up to 16 columns at a time (of 32: 8, and the references fetched again)
+                constexpr int kGroup = RC <= 16 ? RC : 8;
 #pragma unroll
                 for (int y = 0; y < RC; y += kGroup) {
-                    uint32_t pk[3][kGroup / 2];
+                    uint32_t pk[NP][kGroup / 2];
+                    if constexpr (RC > 16) {
+#pragma unroll
+                        for (int r = 0; r < kGroup; r++) ref[y + r] = sb.ref[g][y + r];
+                    }
 #pragma unroll
                     for (int r = 0; r < kGroup; r += 2) {
-                        float e0 = ex2(x[y + r] - sb.ref[g][y + r]), e1 = ex2(x[y + r + 1] - sb.ref[g][y + r + 1]);
+                        float e0 = ex2(x[y + r] - ref[y + r]), e1 = ex2(x[y + r + 1] - ref[y + r + 1]);
                         l[y + r] += e0;
                         l[y + r + 1] += e1;
                         uint32_t h = pack_bf16(e0, e1);
                         pk[0][r / 2] = h;
-                        e0 -= bf16lo(h); e1 -= bf16hi(h);
-                        h = pack_bf16(e0, e1);
-                        pk[1][r / 2] = h;
-                        e0 -= bf16lo(h); e1 -= bf16hi(h);
-                        pk[2][r / 2] = pack_bf16(e0, e1);
+#pragma unroll
+                        for (int t = 1; t < NP; t++) {
+                            e0 -= bf16lo(h); e1 -= bf16hi(h);
+                            h = pack_bf16(e0, e1);
+                            pk[t][r / 2] = h;
+                        }
                     }
 #pragma unroll
-                    for (int t = 0; t < 3; t++) {
-                        if (t < a.p_terms) {
-                            const uint32_t at = p_row + (((t * (RP / 8) + y / 8) ^ (row & 7)) << 4);
-                            if constexpr (RC == 4) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(pk[t][0]), "r"(pk[t][1]) : "memory");
-                            else asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(pk[t][0]), "r"(pk[t][1]), "r"(pk[t][2]), "r"(pk[t][3]) : "memory");
+                    for (int t = 0; t < NP; t++) {
+                        if constexpr (RC == 4) {
+                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(p_row + (((t * (RP / 8)) ^ (row & 7)) << 4)), "r"(pk[t][0]), "r"(pk[t][1]) : "memory");
+                        } else {
+#pragma unroll
+                            for (int z = 0; z < kGroup; z += 8)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p_row + (((t * (RP / 8) + (y + z) / 8) ^ (row & 7)) << 4)),
+                                             "r"(pk[t][z / 2]), "r"(pk[t][z / 2 + 1]), "r"(pk[t][z / 2 + 2]), "r"(pk[t][z / 2 + 3]) : "memory");
                         }
                     }
                 }
@@ -519,58 +544,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
             if (quit) break;
             k += sg.i1 - sg.i0;
 
-            // ---- end of the segment: both groups leave their sums in shared memory, group 0 joins and stores them.  (Loops that
-            // are not unrolled on purpose: this code is cold, and fetching it costs more than running it.)
+            // ---- end of the segment: the group leaves its sums in shared memory
             ok = jg == 0 || mbar_wait(&sb.pv_done[g], (cg - 1) & 1, abort_flag);
             if (ok && seg > 0) ok = mbar_wait(&sb.x_free, (seg - 1) & 1, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
-            tc_fence_after();
-            if (ok && jg > 0) tmem_terms<RC, RP, true>(o_at, a.p_terms, acc);
-            tc_fence_before();
-            if (ok) {
-                const float s = column_sum<RC>(l, lane);
-                if (lane < RC) sb.wsum[g][w][lane] = s;
-                if (has_d) {
-#pragma unroll
-                    for (int r = 0; r < RC; r++) s_x[(g * RC + r) * D + d] = acc[r];
-                }
-                if (row < RC) sb.xref[g][row] = jg == 0 ? kUnset : sb.ref[g][row];
-            }
             if (group_any(g, !ok)) break;
-            if (g == 1) {
-                if (lane == 0) mbar_arrive(&sb.x_ready);
-            } else {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sb.x_ready, seg & 1, abort_flag));
-                if (group_any(g, !ok)) break;
-                constexpr int W = D + 4;
-                float *rec = sg.flags & 1 ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * kRecRows * W;
-                if (row < sg.R) {
-                    const int r = row;
-                    const float r0 = sb.xref[0][r], r1 = sb.xref[1][r];
-                    const float s0 = (sb.wsum[0][0][r] + sb.wsum[0][1][r]) + (sb.wsum[0][2][r] + sb.wsum[0][3][r]);
-                    const float s1 = (sb.wsum[1][0][r] + sb.wsum[1][1][r]) + (sb.wsum[1][2][r] + sb.wsum[1][3][r]);
-                    const float M = fmaxf(r0, r1), m = M == kUnset ? -INFINITY : M;
-                    const float f0 = ex2(r0 - M), f1 = ex2(r1 - M);
-                    const float L = s0 * f0 + s1 * f1, inv = L > 0.f ? 1.f / L : 0.f;
-                    const int64_t orow = tree_out_row(p, sg.b, sg.kvh, r);
-                    sb.join[r] = make_float2(f0 * inv, f1 * inv);
-                    sb.orow[r] = orow;
-                    if (rec) *reinterpret_cast<float4 *>(rec + r * W + D) = make_float4(m * kLn2, L, 0.f, 0.f);
-                    else store_row_stats<D>(p, orow, m, L);
-                }
-                group_any(g, false);
-#pragma unroll 1
-                for (int e = row; e < sg.R * (D / 4); e += 128) {
-                    const int r = e / (D / 4), col = e % (D / 4) * 4;
-                    const float2 f = sb.join[r];
-                    const float4 o0 = *reinterpret_cast<const float4 *>(s_x + r * D + col), o1 = *reinterpret_cast<const float4 *>(s_x + (RC + r) * D + col);
-                    const float4 v = make_float4(o0.x * f.x + o1.x * f.y, o0.y * f.x + o1.y * f.y, o0.z * f.x + o1.z * f.y, o0.w * f.x + o1.w * f.y);
-                    if (rec) *reinterpret_cast<float4 *>(rec + r * W + col) = v;
-                    else store_row4<D>(p, sb.orow[r], col, v);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sb.x_free);
+            tc_fence_after();
+            if (jg > 0) tmem_terms<RC, RP, NP, true>(o_at, acc);
+            tc_fence_before();
+            const float s = column_sum<RC>(l, lane);
+            if (lane < RC) sb.wsum[g][w][lane] = s;
+            if (has_d) {
+#pragma unroll
+                for (int r = 0; r < RC; r++) s_x[(g * RC + r) * D + d] = acc[r];
             }
+            if (row < RC) sb.xref[g][row] = jg == 0 ? kUnset : sb.ref[g][row];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sb.x_ready);
         }
     }
 
@@ -586,28 +576,39 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
 
 constexpr size_t kSmemMost = 227 * 1024 - (sizeof(Bars) + 1023) / 1024 * 1024 - 1024;     // dynamic: beside Bars, and 1024 bytes to align
 
-template <int D, int RC>
-cudaError_t launch_rc(const TreeParams &p, TcArgs &a, cudaStream_t st) {
+template <int D, int RC, int NQ, int NP>
+cudaError_t launch_terms(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     constexpr int RP = RC <= 16 ? 16 : 32;
     static bool ready[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    const size_t slot = kTile * D * 2, rest = 2 * kPBytes + 2 * (size_t)(RP * a.q_terms * D * 2) + 2 * RC * D * sizeof(float);
+    constexpr size_t slot = kTile * D * 2, rest = 2 * kPBytes + 2 * (size_t)(RP * NQ * D * 2) + 2 * RC * D * sizeof(float);
     // an even number: a slot is K's or V's for good, so that its barriers have one producer and one consumer, each of which waits for
     // every phase in turn (a barrier's parity says nothing to one that skips phases)
-    const int slots = (int)((kSmemMost - rest) / slot);
+    constexpr int slots = (int)((kSmemMost - rest) / slot);
+    static_assert(slots >= 4, "two slots each of K and V");
     a.stages = slots > kMaxSlots ? kMaxSlots : slots & ~1;
     if (dev >= 64 || !ready[dev]) {
-        e = cudaFuncSetAttribute(tree_narrow_kernel<D, RC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMost + 1024));
+        e = cudaFuncSetAttribute(tree_narrow_kernel<D, RC, NQ, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMost + 1024));
         if (e != cudaSuccess) return e;
         if (dev < 64) ready[dev] = true;
     }
-    return launch_dependent(tree_narrow_kernel<D, RC>, dim3(sm_count()), kThreads, a.stages * slot + rest + 1024, st, p, a);
+    return launch_dependent(tree_narrow_kernel<D, RC, NQ, NP>, dim3(sm_count()), kThreads, a.stages * slot + rest + 1024, st, p, a);
+}
+template <int D, int RC>
+cudaError_t launch_rc(const TreeParams &p, TcArgs &a, cudaStream_t st) {
+    if (a.p_terms == 3) return a.q_terms == 3 ? launch_terms<D, RC, 3, 3>(p, a, st) : launch_terms<D, RC, 1, 3>(p, a, st);
+    return a.q_terms == 3 ? launch_terms<D, RC, 3, 2>(p, a, st) : launch_terms<D, RC, 1, 2>(p, a, st);
 }
 template <int D> cudaError_t launch_narrow_d(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     const int R = p.n * p.G;
-    return R <= 4 ? launch_rc<D, 4>(p, a, st) : (R <= 8 ? launch_rc<D, 8>(p, a, st) : (R <= 16 ? launch_rc<D, 16>(p, a, st) : launch_rc<D, 32>(p, a, st)));
+    if (R > 16) {
+        if constexpr (D == 64)
+            if (a.q_terms == 3) return launch_terms<D, 32, 3, 2>(p, a, st);
+        return launch_terms<D, 32, 1, 2>(p, a, st);
+    }
+    return R <= 4 ? launch_rc<D, 4>(p, a, st) : (R <= 8 ? launch_rc<D, 8>(p, a, st) : launch_rc<D, 16>(p, a, st));
 }
 
 }  // namespace

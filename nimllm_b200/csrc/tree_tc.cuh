@@ -2,7 +2,7 @@
 //
 // All tiles of a batch are one list ordered by (sequence, KV head, query tile, row), cut into equal spans, one per CTA (one CTA
 // per SM).  A CTA cuts at most two (sequence, KV head, query tile) triples; their pieces go to its two record slots of `recs` and
-// tree_tc_join_kernel finds them by the same arithmetic.
+// tree_finish_kernel (tree_finish.cuh) finds them by the same arithmetic.
 #pragma once
 #include "tcgen05.cuh"
 #include "tree_decode.cuh"
@@ -13,7 +13,8 @@ namespace treetc {
 constexpr int kRecRows = 128;          // query rows of a record slot
 
 struct TcArgs {
-    int64_t *cum;              // [B + 1] units before each sequence, written by CTA 0 for the join
+    int64_t *cum;              // [B + 1] units before each sequence, written by CTA 0 for the finishing launch
+    int4 *starts;              // per CTA: sequence, (KV head, q tile), tile of its first unit
     int q_terms, p_terms, stages;
 };
 
@@ -122,6 +123,7 @@ __device__ __forceinline__ int span_begin(const TreeParams &p, const TcArgs &a, 
         }
     }
     __syncthreads();
+    if (threadIdx.x == 0) a.starts[blockIdx.x] = make_int4(start.b, start.h, start.i, 0);
     return (int)(first_unit(blockIdx.x + 1, T, wa) - u0);
 }
 
