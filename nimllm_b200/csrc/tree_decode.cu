@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(256) tree_fma_kernel(TreeParams p) {
         }
     if (c8 == 0) {
         if (rec) *reinterpret_cast<float4 *>(rec + D) = make_float4(m * kLn2, l, 0.f, 0.f);
-        if (n_chunks == 1 && p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(m, inv);
+        if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(m, n_chunks == 1 ? inv : -1.f);   // -1: cut
     }
 }
 

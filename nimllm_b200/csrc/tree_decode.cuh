@@ -1,4 +1,4 @@
-// tree_decode.cuh -- what the kernels of tree_decode.cu and tree_decode_tc.cu share.
+// tree_decode.cuh -- what the kernels of tree_decode.cu and tree_wide_tc.cu share.
 #pragma once
 #include "cache_rows.cuh"
 
@@ -52,7 +52,7 @@ __device__ __forceinline__ int64_t tree_out_row(const TreeParams &p, int b, int 
     return ((int64_t)b * p.n + i) * p.Hq + kvh * p.G + (qr - i * p.G);
 }
 
-// the tensor-core kernel for bf16 caches (tree_decode_tc.cu)
+// the tensor-core kernel for bf16 caches (tree_wide_tc.cu)
 size_t tree_tc_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim);
 int launch_tree_tc(const char *who, TreeParams &p, int head_dim, void *workspace, cudaStream_t st);
 

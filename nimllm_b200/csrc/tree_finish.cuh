@@ -36,9 +36,9 @@ template <int D> __device__ __forceinline__ Pieces tc_pieces(const TreeParams &p
     const int64_t s = f.tc.cum[b] + ((int64_t)kvh * q_tiles + qt) * tiles;
     const int w0 = owner_of(s, T, wa);
     x.n = owner_of(s + tiles - 1, T, wa) - w0 + 1;
-    x.step = (int64_t)2 * kRecRows * W;
-    x.first = p.recs + ((int64_t)w0 * 2 + (first_unit(w0, T, wa) < s ? 1 : 0)) * kRecRows * W + r * W;
-    x.second = p.recs + ((int64_t)(w0 + 1) * 2) * kRecRows * W + r * W;
+    x.step = (int64_t)2 * f.tc.rec_rows * W;
+    x.first = p.recs + ((int64_t)w0 * 2 + (first_unit(w0, T, wa) < s ? 1 : 0)) * f.tc.rec_rows * W + r * W;
+    x.second = p.recs + ((int64_t)(w0 + 1) * 2) * f.tc.rec_rows * W + r * W;
     return x;
 }
 template <int D> __device__ __forceinline__ Pieces chunk_pieces(const TreeParams &p, int64_t orow, int total) {
@@ -98,11 +98,11 @@ template <int D> __device__ __forceinline__ void join_row(const TreeParams &p, c
         if (p.out) store_from_f32(p.out, p.out_dtype, orow * D + d, acc[j]);
         if (p.partials_out) p.partials_out[orow * (D + 4) + d] = acc[j];
     }
-    if (lane == 0) store_row_stats<D>(p, orow, M * kLog2e, L);
+    if (lane == 0 && p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + D) = make_float4(M, L, 0.f, 0.f);
 }
 
 template <int D>
-__global__ void __launch_bounds__(kFinishThreads) tree_finish_kernel(TreeParams p, FinishArgs f) {
+__global__ void __launch_bounds__(kFinishThreads, 5) tree_finish_kernel(TreeParams p, FinishArgs f) {
     __shared__ float2 s_stat[256];
     launch_dependents();
     grid_dependency_wait();
@@ -155,47 +155,59 @@ __global__ void __launch_bounds__(kFinishThreads) tree_finish_kernel(TreeParams 
         return;
     }
     x -= f.n_zero;
-    // score[r] = decay * score[r] + sum over the G heads of exp2(raw - m) / l, four rows a thread
+    // score[r] = decay * score[r] + sum over the G heads of exp2(raw - m) / l, four rows a thread.  What a block reads first -- length,
+    // statistics, raw scores, old scores -- has addresses that depend on nothing, so that its loads wait for memory together.
     const int blocks = (p.max_len + kScoreRows - 1) / kScoreRows;
     const int pair = x / blocks, b = pair / p.Hkv, kvh = pair - b * p.Hkv;
-    const int len = tree_committed(p, b), r0 = (x - pair * blocks) * kScoreRows;
+    const int r0 = (x - pair * blocks) * kScoreRows, row = r0 + threadIdx.x * 4;
+    const int64_t h0 = (int64_t)b * p.Hq + kvh * p.G;
+    const float *raw = p.raw + h0 * p.raw_ld + row;
+    constexpr int kAhead = 4;
+    float4 ahead[kAhead];
+    const bool in_raw = row < p.max_len;                   // the workspace holds whole rows of scores, whatever the length
+#pragma unroll
+    for (int g = 0; g < kAhead; g++) ahead[g] = in_raw && g < p.G ? __ldcs(reinterpret_cast<const float4 *>(raw + g * p.raw_ld)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float *s = p.score + ((int64_t)b * p.Hkv + kvh) * p.score_rows + row;
+    float old[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) old[j] = p.decay != 0.f && row + j < p.max_len ? s[j] : 0.f;
+    float2 st = make_float2(0.f, 0.f);
+    if ((int)threadIdx.x < min(256, p.G)) st = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + threadIdx.x));
+    const int len = tree_committed(p, b);
     if (r0 >= len) return;
-    const int row = r0 + threadIdx.x * 4;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int g0 = 0; g0 < p.G; g0 += 256) {
         const int n = min(256, p.G - g0);
-        __syncthreads();
-        for (int g = warp; g < n; g += 8) {
-            const int64_t h = (int64_t)b * p.Hq + kvh * p.G + g0 + g;
-            const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g0 + g, len, p.G) : chunk_pieces<D>(p, h, len);
-            float2 st;
-            if (pc.n > 1) {
+        if (g0) {
+            __syncthreads();
+            if ((int)threadIdx.x < n) st = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + g0 + threadIdx.x));
+        }
+        if ((int)threadIdx.x < n) s_stat[threadIdx.x] = st;
+        // a negative sum marks a row that was cut: its pieces are joined here
+        if (__syncthreads_or((int)threadIdx.x < n && st.y < 0.f)) {
+            for (int g = warp; g < n; g += 8) {
+                const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g0 + g, len, p.G) : chunk_pieces<D>(p, h0 + g0 + g, len);
                 float M, L;
                 pieces_stats<D>(pc, lane, M, L);
-                st = make_float2(M * kLog2e, L > 0.f ? 1.f / L : 0.f);
-            } else {
-                st = *reinterpret_cast<const float2 *>(p.stats + 2 * h);
+                if (lane == 0) s_stat[g] = make_float2(M * kLog2e, L > 0.f ? 1.f / L : 0.f);
             }
-            if (lane == 0) s_stat[g] = st;
+            __syncthreads();
         }
-        __syncthreads();
         if (row < len) {
-            const float *raw = p.raw + ((int64_t)b * p.Hq + kvh * p.G + g0) * p.raw_ld + row;
 #pragma unroll 4
             for (int g = 0; g < n; g++) {
-                const float4 s = *reinterpret_cast<const float4 *>(raw + g * p.raw_ld);
-                const float2 st = s_stat[g];
-                sum[0] += ex2(s.x - st.x) * st.y; sum[1] += ex2(s.y - st.x) * st.y;
-                sum[2] += ex2(s.z - st.x) * st.y; sum[3] += ex2(s.w - st.x) * st.y;
+                const float4 v = g0 == 0 && g < kAhead ? ahead[g & (kAhead - 1)] : *reinterpret_cast<const float4 *>(raw + (g0 + g) * p.raw_ld);
+                const float2 t = s_stat[g];
+                sum[0] += ex2(v.x - t.x) * t.y; sum[1] += ex2(v.y - t.x) * t.y;
+                sum[2] += ex2(v.z - t.x) * t.y; sum[3] += ex2(v.w - t.x) * t.y;
             }
         }
     }
     // the four rows lie in one page (page_rows >= 32); without a page they have no raw score
     if (row >= len || (p.rows.table && cache_row(p.rows, b, kvh, row) < 0)) return;
-    float *s = p.score + ((int64_t)b * p.Hkv + kvh) * p.score_rows + row;
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (row + j < len) s[j] = (p.decay == 0.f ? 0.f : p.decay * s[j]) + sum[j];
+        if (row + j < len) s[j] = (p.decay == 0.f ? 0.f : p.decay * old[j]) + sum[j];
 }
 
 template <int D> inline cudaError_t launch_finish(const TreeParams &p, FinishArgs &f, cudaStream_t st) {

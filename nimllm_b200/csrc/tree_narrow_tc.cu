@@ -4,11 +4,11 @@
 //     S^T = K Q^T     (128 cached rows x N, one thread per cached row)
 //     O^T += V^T P^T  (head_dim x N, A = V as it lies in the cache, B = P^T written to shared memory by the softmax)
 // and N is the query rows, 16 or 32, times the bf16 terms of an fp32 q (S) or of P (O): the terms are further columns of the
-// same MMA, so that 32-bit precision costs little tensor time.  (tree_decode_tc.cu has the terms' sizes.)
+// same MMA, so that 32-bit precision costs little tensor time.  (tree_wide_tc.cu has the terms' sizes.)
 //
 //   warps 0-3, 4-7   two softmax groups, taking the tiles of 128 rows in turn: the waits of one hide behind the other
 //   warps 8-11       K rows (8, 9) and V rows (10, 11) into a ring of slots with cp.async, swizzled, exact to the row
-//                    (tree_decode_tc.cu says why no TMA)
+//                    (tree_wide_tc.cu says why no TMA)
 //   warp 12          walks the CTA's span and hands its segments to the others; Q of the segments to come (two buffers), and which
 //                    query rows see each of their drafts
 //   warps 13, 14     issue K Q^T and V^T P^T, each in order and waiting for its own operands alone
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
         constexpr int W = D + 4;
         for (int seg = 0; next_segment(sb, seg, sg, ok, lane); seg++) {
             if (!(ok = __all_sync(0xffffffffu, mbar_wait(&sb.x_ready, seg & 1, abort_flag)))) break;
-            float *rec = sg.flags & 1 ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * kRecRows * W;
+            float *rec = sg.flags & 1 ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * a.rec_rows * W;
             if (lane < sg.R) {                             // lane r: how much of each group's O counts
                 const int r = lane;
                 const float r0 = sb.xref[0][r], r1 = sb.xref[1][r];
@@ -373,8 +373,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                 const int64_t orow = tree_out_row(p, sg.b, sg.kvh, r);
                 sb.join[r] = make_float2(f0 * inv, f1 * inv);
                 sb.orow[r] = orow;
-                if (rec) *reinterpret_cast<float4 *>(rec + r * W + D) = make_float4(m * kLn2, L, 0.f, 0.f);
-                else store_row_stats<D>(p, orow, m, L);
+                if (rec) {
+                    *reinterpret_cast<float4 *>(rec + r * W + D) = make_float4(m * kLn2, L, 0.f, 0.f);
+                    mark_cut(p, orow);
+                } else {
+                    store_row_stats<D>(p, orow, m, L);
+                }
             }
             __syncwarp();
 #pragma unroll 2

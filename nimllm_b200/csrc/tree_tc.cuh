@@ -10,12 +10,11 @@
 namespace nimllm {
 namespace treetc {
 
-constexpr int kRecRows = 128;          // query rows of a record slot
-
 struct TcArgs {
     int64_t *cum;              // [B + 1] units before each sequence, written by CTA 0 for the finishing launch
     int4 *starts;              // per CTA: sequence, (KV head, q tile), tile of its first unit
     int q_terms, p_terms, stages;
+    int rec_rows;              // query rows of a record slot
 };
 
 __host__ __device__ inline int64_t first_unit(int w, int64_t T, int wa) { return (int64_t)w * T / wa; }
@@ -146,13 +145,27 @@ __device__ __forceinline__ void store_row4(const TreeParams &p, int64_t orow, in
     }
     if (p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + d) = x;
 }
+// eight columns: 16 bytes of a bf16 row
+template <int D>
+__device__ __forceinline__ void store_row8(const TreeParams &p, int64_t orow, int d, const float *x) {
+    if (p.out && p.out_dtype == NIMLLM_BF16 && !p.partials_out) {
+        *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + orow * D + d) =
+            make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    } else {
+        store_row4<D>(p, orow, d, make_float4(x[0], x[1], x[2], x[3]));
+        store_row4<D>(p, orow, d + 4, make_float4(x[4], x[5], x[6], x[7]));
+    }
+}
 template <int D>
 __device__ __forceinline__ void store_row_stats(const TreeParams &p, int64_t orow, float m, float l) {
     if (p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + D) = make_float4(m * kLn2, l, 0.f, 0.f);
     if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(m, l > 0.f ? 1.f / l : 0.f);
 }
 
-inline size_t rec_bytes(int head_dim) { return (size_t)sm_count() * 2 * kRecRows * rec_stride(head_dim) * sizeof(float); }
+// a row that was cut has no statistics yet: the score blocks join its pieces themselves
+__device__ __forceinline__ void mark_cut(const TreeParams &p, int64_t orow) {
+    if (p.stats) p.stats[2 * orow + 1] = -1.f;
+}
 
 // tree_narrow_tc.cu: few query rows
 bool tree_narrow_takes(int R, int q_terms, int p_terms, int head_dim);
