@@ -276,8 +276,9 @@ int nimllm_rope_at_bwd(const void *dq_rot, void *dq, int n_head, const void *dk_
  *   tree_mask  device uint64 [batch, n, (n + 63) / 64]: bit j of token i's words, it attends draft j (its
  *              ancestors and itself); NULL: a chain, drafts 0 .. i.  A token without any row to attend gets zeros
  *   partials_out  optional fp32 [batch*n*n_head, head_dim + 4] records as in nimllm_attn_decode (out may be NULL then)
- *   head_dim   64 or 128.  The products are those of 32-bit arithmetic for either cache type; every row of V up to the last
- *              draft must be finite even where a mask hides it (a hidden row of K may hold anything)
+ *   head_dim   64 or 128.  The arithmetic is that of 32 bits for either cache type, but for bf16 results of more than 32
+ *              query rows (n * n_head / n_kv_head), whose softmax weights are rounded to bf16.  Every row of V up to the
+ *              last draft must be finite even where a mask hides it (a hidden row of K may hold anything)
  *   workspace  256-byte aligned, nimllm_attn_decode_tree_workspace_bytes(...) bytes
  * The kernel for bf16 caches (also that of nimllm_attn_decode_scored) bounds its internal waits, about 2 s without
  * progress; nimllm_attn_decode_tree_status tells as nimllm_attn_prefill_status does whether one gave up. */

@@ -163,6 +163,8 @@ __global__ void __launch_bounds__(256) tree_fma_kernel(TreeParams p) {
 int tree_chunk_rows(int batch, int n, int n_head, int n_kv_head, int max_total) {
     const int64_t tiles = (int64_t)batch * n_kv_head * (((int64_t)n * (n_head / n_kv_head) + kBM - 1) / kBM);
     int64_t c = (tiles * max_total + 4 * sm_count() - 1) / (4 * sm_count());
+    const int64_t least = ((int64_t)max_total + treetc::kMaxPieces - 1) / treetc::kMaxPieces;
+    c = c < least ? least : c;
     c = (c + kBN - 1) / kBN * kBN;
     return (int)(c < 128 ? 128 : (c > (1 << 30) ? 1 << 30 : c));
 }

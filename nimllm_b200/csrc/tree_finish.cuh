@@ -10,6 +10,7 @@ namespace nimllm {
 namespace treetc {
 
 constexpr int kFinishThreads = 256, kScoreRows = 4 * kFinishThreads;
+constexpr int kMaxPieces = 180;        // 32 rows of them in 48 KB
 
 // The pieces of a query row.  Tensor-core kernels: records of consecutive CTAs (tree_tc.cuh); CUDA-core kernel: one record per chunk of
 // rows.  n = 1: the kernel stored the row itself; n = 0: there was nothing to attend.
@@ -22,7 +23,7 @@ struct Pieces {
 struct FinishArgs {
     TcArgs tc;
     int rpt, tile, workers;            // tensor-core kernels; workers = 0: the chunks of the CUDA-core kernel
-    int join_rows, n_join, n_zero, n_score;   // query rows of a join block; blocks of the three kinds
+    int n_join, n_zero;                // blocks of the first two kinds
 };
 
 template <int D> __device__ __forceinline__ Pieces tc_pieces(const TreeParams &p, const FinishArgs &f, int b, int kvh, int qr, int total, int R) {
@@ -70,69 +71,84 @@ template <int D> __device__ __forceinline__ void pieces_stats(const Pieces &x, i
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
 }
 
-// one warp: the row that its pieces make
-template <int D> __device__ __forceinline__ void join_row(const TreeParams &p, const Pieces &x, int64_t orow, int lane) {
-    float M, L;
-    pieces_stats<D>(x, lane, M, L);
-    const float safe = M == -INFINITY ? 0.f : M, inv = L > 0.f ? 1.f / L : 0.f;
-    constexpr int V = D / 32;                              // columns of a lane, side by side
-    float acc[V];
+// One block joins up to 32 rows that are cut alike: piece i of row r is the record at rec(i) + r * W.  `out_row(r)` is its row of out.
+// First every (row, piece) statistic is fetched at once and turned into the piece's weight, then every 16 bytes of the rows is a sum
+// over the pieces whose loads wait for nothing else.
+constexpr int kJoinRows = 32;
+template <int D, typename OutRow>
+__device__ __forceinline__ void join_rows(const TreeParams &p, const Pieces &x, int rows, OutRow out_row, float2 *s_ml) {
+    constexpr int W = D + 4, kLanes = kFinishThreads / kJoinRows;
+    for (int e = threadIdx.x; e < rows * x.n; e += kFinishThreads) {
+        const int i = e / rows, r = e - i * rows;
+        s_ml[r * x.n + i] = *reinterpret_cast<const float2 *>(x.rec(i) + r * W + D);
+    }
+    __syncthreads();
+    const int r = threadIdx.x / kLanes, sub = threadIdx.x % kLanes;
+    if (r < rows) {                                        // eight threads of one warp per row
+        float2 *ml = s_ml + r * x.n;
+        const unsigned mask = 0xffu << (threadIdx.x & 24);
+        float M = -INFINITY, L = 0.f;
+        for (int i = sub; i < x.n; i += kLanes)
+            if (ml[i].y > 0.f) M = fmaxf(M, ml[i].x);
 #pragma unroll
-    for (int j = 0; j < V; j++) acc[j] = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < x.n; i++) {
-        const float *rec = x.rec(i);
-        const float2 ml = *reinterpret_cast<const float2 *>(rec + D);
-        const float w = ml.y > 0.f ? ml.y * ex2((ml.x - safe) * kLog2e) * inv : 0.f;
-        if constexpr (V == 4) {
-            const float4 o = *reinterpret_cast<const float4 *>(rec + lane * 4);
-            acc[0] = fmaf(w, o.x, acc[0]); acc[1] = fmaf(w, o.y, acc[1]); acc[2] = fmaf(w, o.z, acc[2]); acc[3] = fmaf(w, o.w, acc[3]);
-        } else {
-            const float2 o = *reinterpret_cast<const float2 *>(rec + lane * 2);
-            acc[0] = fmaf(w, o.x, acc[0]); acc[1] = fmaf(w, o.y, acc[1]);
+        for (int off = kLanes / 2; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(mask, M, off));
+        const float safe = M == -INFINITY ? 0.f : M;
+        for (int i = sub; i < x.n; i += kLanes) {
+            const float w = ml[i].y > 0.f ? ml[i].y * ex2((ml[i].x - safe) * kLog2e) : 0.f;
+            ml[i].x = w;
+            L += w;
         }
-    }
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        const int d = lane * V + j;
-        if (p.out) store_from_f32(p.out, p.out_dtype, orow * D + d, acc[j]);
-        if (p.partials_out) p.partials_out[orow * (D + 4) + d] = acc[j];
+        for (int off = kLanes / 2; off > 0; off >>= 1) L += __shfl_xor_sync(mask, L, off);
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        for (int i = sub; i < x.n; i += kLanes) ml[i].x *= inv;
+        if (sub == 0 && p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + out_row(r) * W + D) = make_float4(M, L, 0.f, 0.f);
     }
-    if (lane == 0 && p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + D) = make_float4(M, L, 0.f, 0.f);
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * (D / 4); e += kFinishThreads) {
+        const int rr = e / (D / 4), d = e % (D / 4) * 4;
+        const float2 *w = s_ml + rr * x.n;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < x.n; i++) {
+            const float4 o = *reinterpret_cast<const float4 *>(x.rec(i) + rr * W + d);
+            const float f = w[i].x;
+            acc.x = fmaf(f, o.x, acc.x); acc.y = fmaf(f, o.y, acc.y); acc.z = fmaf(f, o.z, acc.z); acc.w = fmaf(f, o.w, acc.w);
+        }
+        store_row4<D>(p, out_row(rr), d, acc);
+    }
 }
 
 template <int D>
 __global__ void __launch_bounds__(kFinishThreads, 5) tree_finish_kernel(TreeParams p, FinishArgs f) {
-    __shared__ float2 s_stat[256];
+    extern __shared__ float2 s_dyn[];                      // join: kJoinRows x pieces; score: 256 heads
+    float2 *s_stat = s_dyn;
     launch_dependents();
     grid_dependency_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int x = blockIdx.x;
     if (x < f.n_join) {
         if (f.workers == 0) {
-            // rows of out, eight a block
-            const int64_t orow = (int64_t)x * 8 + warp;
-            if (orow >= (int64_t)p.B * p.n * p.Hq) return;
-            const int b = (int)(orow / ((int64_t)p.n * p.Hq)), i = (int)(orow / p.Hq % p.n);
-            if (i >= tree_tokens(p, b)) return;
+            // 32 rows of a sequence's results
+            const int per = (p.n * p.Hq + kJoinRows - 1) / kJoinRows, b = x / per, first = (x - b * per) * kJoinRows;
+            const int rows = min(kJoinRows, tree_tokens(p, b) * p.Hq - first);
             const int len = tree_committed(p, b);
+            const int64_t orow = (int64_t)b * p.n * p.Hq + first;
             const Pieces pc = chunk_pieces<D>(p, orow, len + tree_drafts(p, b, len));
-            if (pc.n > 1) join_row<D>(p, pc, orow, lane);
+            if (rows > 0 && pc.n > 1) join_rows<D>(p, pc, rows, [&](int r) { return orow + r; }, s_dyn);
             return;
         }
         // the pair whose first cut is where CTA w begins; `per` blocks share its rows
-        const int per = f.rpt / f.join_rows, w = x / per + 1, r_first = (x % per) * f.join_rows;
+        const int per = f.rpt / kJoinRows, w = x / per + 1, first = (x % per) * kJoinRows;
         const int64_t T = f.tc.cum[p.B];
+        const int4 at = f.tc.starts[w];                    // sequence, KV head and q tile, tile (not written past the last worker)
         const int wa = (int)(T < f.workers ? T : f.workers);
-        if (w >= wa) return;
-        const int4 at = f.tc.starts[w];                    // sequence, KV head and q tile, tile
-        if (at.z == 0 || owner_of(first_unit(w, T, wa) - at.z, T, wa) != w - 1) return;
+        if (w >= wa || at.z == 0 || owner_of(first_unit(w, T, wa) - at.z, T, wa) != w - 1) return;
         const int len = tree_committed(p, at.x), total = len + tree_drafts(p, at.x, len), R = tree_tokens(p, at.x) * p.G;
-        const int q_tiles = (R + f.rpt - 1) / f.rpt, kvh = at.y / q_tiles, qt = at.y - kvh * q_tiles;
-        for (int r = r_first + warp; r < r_first + f.join_rows && qt * f.rpt + r < R; r += 8) {
-            const int qr = qt * f.rpt + r;
-            join_row<D>(p, tc_pieces<D>(p, f, at.x, kvh, qr, total, R), tree_out_row(p, at.x, kvh, qr), lane);
-        }
+        const int q_tiles = (R + f.rpt - 1) / f.rpt, kvh = at.y / q_tiles, q0 = (at.y - kvh * q_tiles) * f.rpt + first;
+        const int rows = min(kJoinRows, R - q0);
+        if (rows > 0)
+            join_rows<D>(p, tc_pieces<D>(p, f, at.x, kvh, q0, total, R), rows, [&](int r) { return tree_out_row(p, at.x, kvh, q0 + r); }, s_dyn);
         return;
     }
     x -= f.n_join;
@@ -211,19 +227,22 @@ __global__ void __launch_bounds__(kFinishThreads, 5) tree_finish_kernel(TreePara
 }
 
 template <int D> inline cudaError_t launch_finish(const TreeParams &p, FinishArgs &f, cudaStream_t st) {
+    size_t pieces;
     if (f.workers) {
-        f.join_rows = f.rpt < 8 ? f.rpt : 8;
-        f.n_join = (f.workers - 1) * (f.rpt / f.join_rows);
+        f.n_join = (f.workers - 1) * (f.rpt / kJoinRows);
         f.n_zero = (p.B + 31) / 32;
+        pieces = f.workers;
     } else {
-        f.n_join = p.max_chunks > 1 ? (int)(((int64_t)p.B * p.n * p.Hq + 7) / 8) : 0;
+        f.n_join = p.max_chunks > 1 ? p.B * ((p.n * p.Hq + kJoinRows - 1) / kJoinRows) : 0;
         f.n_zero = 0;
+        pieces = p.max_chunks;
     }
-    f.n_score = p.score ? p.B * p.Hkv * ((p.max_len + kScoreRows - 1) / kScoreRows) : 0;
     const int64_t blocks = (int64_t)f.n_join + f.n_zero + (p.score ? (int64_t)p.B * p.Hkv * ((p.max_len + kScoreRows - 1) / kScoreRows) : 0);
     if (blocks == 0) return cudaSuccess;
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    return launch_dependent(tree_finish_kernel<D>, dim3((unsigned)blocks), kFinishThreads, 0, st, p, f);
+    if (blocks > 0x7fffffff || pieces > kMaxPieces) return cudaErrorInvalidConfiguration;
+    size_t smem = f.n_join ? kJoinRows * pieces * sizeof(float2) : 0;
+    if (smem < 256 * sizeof(float2)) smem = 256 * sizeof(float2);
+    return launch_dependent(tree_finish_kernel<D>, dim3((unsigned)blocks), kFinishThreads, smem, st, p, f);
 }
 
 }  // namespace treetc

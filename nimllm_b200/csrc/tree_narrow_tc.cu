@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
         const int which = (warp - 8) >> 1, t = (int)threadIdx.x - 256 - which * 64, c = t % kChunks, r_in = t / kChunks;
         const uint32_t kv = smem_u32(s_kv);
         const __nv_bfloat16 *src = reinterpret_cast<const __nv_bfloat16 *>(which ? p.v : p.k) + c * 8;
+        const uint64_t once = evict_first_policy();
         int k = 0, slot = which, phase = 1;
         for (int seg = 0; next_segment(sb, seg, sg, ok, lane); seg++) {
             // the loads of the first Q go out before a ring full of rows queues up in front of them
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                     for (int r0 = 0; r0 < 32; r0 += kStep) {
                         const int rr = y * 32 + r0 + r_in;
                         const bool have = r0 + r_in < r_end;
-                        cp_async16(dst + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), have ? g + r0 * D : src, have ? 16 : 0);
+                        cp_async16(dst + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), have ? g + r0 * D : src, have ? 16 : 0, once);
                     }
                 }
                 cp_async_arrive(&sb.full[slot]);

@@ -130,6 +130,15 @@ __device__ __forceinline__ int span_begin(const TreeParams &p, const TcArgs &a, 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// the same for rows that nobody reads again in this launch: they leave L2 first, so that records, scores and code stay
+__device__ __forceinline__ uint64_t evict_first_policy() {
+    uint64_t pol;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
+    return pol;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes), "l"(policy) : "memory");
+}
 // arrives on the barrier when this thread's copies so far have landed.  The reader of the data is the tensor core: the warp that
 // issues the MMAs orders the copies before them with a proxy fence behind its wait.
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {

@@ -16,10 +16,11 @@
 // ref is a query row's running maximum, taken anew only when a score passes it by more than 2^32: rounding is relative to P's own
 // size, and fp32 has the range.  O is then rescaled in TMEM, which costs nothing while it does not happen.
 //
-// Precision: the products are exact in fp32 accumulation, so the only roundings to bf16 are those of P and of an fp32 q.  Both are
-// split: an fp32 q into three bf16 terms (2^-26 left), P into two terms for bf16 results (2^-17) and three for fp32 results.
-// The terms are further MMAs into the same accumulator.  For fp32 results O is taken from TMEM into registers every few tiles:
-// thousands of rows added up by the tensor core would lose what 32-bit results promise.
+// Precision: the products are exact in fp32 accumulation, so the only roundings to bf16 are those of P and of an fp32 q.  For fp32
+// results both are split into three bf16 terms (2^-26 left), further MMAs into the same accumulator, and O is taken from TMEM into
+// registers every few tiles: thousands of rows added up by the tensor core would lose what 32-bit results promise.  For bf16 results
+// P is rounded to bf16 like the result itself (the sum is taken of the rounded values, so that a single large weight stays exact);
+// a second term would make this kernel, which the tensor pipe bounds, a third slower (64-token trees over 16 K rows: 187 us).
 //
 // Every wait is bounded as in prefill_tc.cu: after about 2 s without progress the CTA aborts and raises the status word.
 #include "tree_finish.cuh"
@@ -52,7 +53,7 @@ struct SegEntry {
 struct Bars {
     uint64_t full[kMaxSlots], empty[kMaxSlots];
     uint64_t seg_full[kSegs], seg_empty[kSegs];
-    uint64_t q_full[2], q_empty[2];
+    uint64_t q_full[2], q_empty[2], q_asked;
     uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2];
     uint64_t x_ready, x_free, drain[2];
     uint32_t tmem_base;
@@ -106,7 +107,7 @@ __device__ __forceinline__ void unpair2(uint64_t v, float &a, float &b) { asm("m
 __device__ __forceinline__ uint64_t add2_f32(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ uint64_t mul2_f32(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
-// 32 scaled scores, less the reference, -> NP terms of P (16 packed columns each); adds the exponentials to l
+// 32 scaled scores, less the reference, -> NP terms of P (16 packed columns each); adds the exponentials (NP = 1: rounded) to l
 template <int NP> __device__ __forceinline__ void exps32(const float *x, float ref, float &l, uint32_t pk[NP][16]) {
     const uint64_t nr = pair2(-ref, -ref);
     uint64_t sum = 0ull;
@@ -117,9 +118,9 @@ template <int NP> __device__ __forceinline__ void exps32(const float *x, float r
         e0 = ex2(e0);
         e1 = ex2(e1);
         uint64_t e = pair2(e0, e1);
-        sum = add2_f32(sum, e);
         uint32_t h = pack_bf16(e0, e1);
         pk[0][y / 2] = h;
+        sum = add2_f32(sum, NP == 1 ? pair2(bf16lo(h), bf16hi(h)) : e);
 #pragma unroll
         for (int t = 1; t < NP; t++) {
             e = add2_f32(e, pair2(-bf16lo(h), -bf16hi(h)));
@@ -149,7 +150,7 @@ __device__ __forceinline__ void hide32(float *x, uint32_t vis) {
         if (!((vis >> y) & 1)) x[y] = -INFINITY;
 }
 
-// NQ, NP: terms of q and of P; SPLIT: 256 query rows a tile, half of them per group (else 128, the tiles in turn)
+// NQ, NP: terms of q (1, 3) and of P (1, 3); SPLIT: 256 query rows a tile, half of them per group (else 128, the tiles in turn)
 template <int D, int NQ, int NP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, TcArgs a) {
     constexpr int RPT = SPLIT ? 2 * kRows : kRows;
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
             mbar_init(&sb.s_full[g], 1); mbar_init(&sb.s_free[g], 4);
             mbar_init(&sb.p_ready[g], 4); mbar_init(&sb.pv_done[g], 1);
         }
-        mbar_init(&sb.x_ready, 4); mbar_init(&sb.x_free, 4); mbar_init(&sb.drain[0], 1); mbar_init(&sb.drain[1], 1);
+        mbar_init(&sb.q_asked, 64); mbar_init(&sb.x_ready, 4); mbar_init(&sb.x_free, 4); mbar_init(&sb.drain[0], 1); mbar_init(&sb.drain[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // rows of the Q tile that no query row fills stay zero (or hold an earlier segment's rows): finite, never used
@@ -203,6 +204,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
         const __nv_bfloat16 *src = reinterpret_cast<const __nv_bfloat16 *>(which ? p.v : p.k) + c * 8;
         int k = 0, slot = which, phase = 1;
         for (int seg = 0; next_segment(sb, seg, sg, ok, lane); seg++) {
+            // the loads of the first Q go out before a ring full of rows queues up in front of them
+            if (seg == 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&sb.q_asked, 0, abort_flag)))) break;
             for (int i = sg.i0; i < sg.i1; i++, k++) {
                 const int t0 = i * kTile, n = min(kTile, sg.total - t0);
                 // a half of a tile lies in one page (page_rows >= 32)
@@ -263,9 +266,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                 for (int r = half * kStep + lane / kChunks; r < rows; r += 2 * kStep)
                     cp_async16(qs + (r >> 7) * kQTile + (c >> 3) * kQBox + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
                                qg + tree_out_row(p, sg.b, sg.kvh, q0 + r) * D, 16);
+                if (seg == 0) mbar_arrive(&sb.q_asked);
                 asm volatile("cp.async.wait_all;" ::: "memory");
             } else {
                 constexpr int kChunks = D / 4, kStep = 32 / kChunks;      // four values a lane
+                static_assert(kStep == 128 / D, "");
                 const int c = lane % kChunks;
                 const float *qg = reinterpret_cast<const float *>(p.q) + c * 4;
                 for (int r0 = half * kStep; r0 < rows; r0 += 16 * kStep) {
@@ -275,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                         const int r = r0 + u * 2 * kStep + lane / kChunks;
                         if (r < rows) x[u] = *reinterpret_cast<const float4 *>(qg + tree_out_row(p, sg.b, sg.kvh, q0 + r) * D);
                     }
+                    if (seg == 0 && r0 == half * kStep) mbar_arrive(&sb.q_asked);
 #pragma unroll
                     for (int u = 0; u < 8; u++) {
                         const int r = r0 + u * 2 * kStep + lane / kChunks;
@@ -292,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                     }
                 }
             }
+            if (NQ > 1 && seg == 0 && half * (128 / D) >= rows) mbar_arrive(&sb.q_asked);      // this warp has no row
             fence_async();
             mbar_arrive(&sb.q_full[buf]);
         }
@@ -645,8 +652,8 @@ cudaError_t launch_d(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     const bool narrow = tree_narrow_takes(R, a.q_terms, a.p_terms, D);
     cudaError_t e;
     if (narrow) e = launch_tree_narrow(p, a, D, st);
-    else if (a.q_terms == 1) e = a.p_terms == 2 ? launch_wide<D, 1, 2>(p, a, st) : launch_wide<D, 1, 3>(p, a, st);
-    else e = a.p_terms == 2 ? launch_wide<D, 3, 2>(p, a, st) : launch_wide<D, 3, 3>(p, a, st);
+    else if (a.q_terms == 1) e = a.p_terms == 2 ? launch_wide<D, 1, 1>(p, a, st) : launch_wide<D, 1, 3>(p, a, st);
+    else e = a.p_terms == 2 ? launch_wide<D, 3, 1>(p, a, st) : launch_wide<D, 3, 3>(p, a, st);
     if (e != cudaSuccess) return e;
     FinishArgs f = {};
     f.tc = a; f.rpt = rows_per_tile(R, a.q_terms, a.p_terms, D); f.tile = narrow ? kNarrowTile : kTile; f.workers = sm_count();

@@ -115,13 +115,15 @@ def attend(q, k, v, see, scale):
     return out.reshape(n, Hq, D), m.view(n, Hq), l.view(n, Hq), w.view(n, Hq, L), float(mag.max())
 
 
-def attention_tolerance(D, rows, mag, v_max, out_dtype):
+def attention_tolerance(D, rows, mag, v_max, out_dtype, wide=False):
     """How far an output may be off.  u = 2^-24.  A score is a sum of D products in 32 bits, then scaled: off by at most
     (D + 3) u mag, which moves every weight by that factor (numerator and sum: twice), the exponential by 2^-22; the sums over
     the rows add rows * u.  A weight is split into three bf16 terms for 32-bit results (2^-26 left) and two for bf16 results
-    (2^-17 left).  The result is a weighted mean of values of at most v_max."""
+    (2^-17 left); bf16 results of more than 32 query rows per KV head (wide) round it once, numerator and sum by 2^-8 each.
+    The result is a weighted mean of values of at most v_max."""
     u = 2.0 ** -24
-    rel = 2 * ((D + 3) * u * mag + 2.0 ** -22) + (rows + 2) * u + (2.0 ** -26 if out_dtype == torch.float32 else 2.0 ** -17)
+    rel = 2 * ((D + 3) * u * mag + 2.0 ** -22) + (rows + 2) * u
+    rel += 2.0 ** -26 if out_dtype == torch.float32 else (2.0 ** -7 if wide else 2.0 ** -17)
     return rel * v_max
 
 
