@@ -4,6 +4,8 @@
 // (16-byte pieces of the rows) of one (sequence, KV head) and walks the destinations upwards in batches: it loads a batch's
 // rows, waits for all of its threads, stores them.  A later batch reads rows src[j] >= j behind everything stored so far, so
 // one barrier per batch is all the order that is needed.
+#include <cooperative_groups.h>
+
 #include "cache_rows.cuh"
 
 namespace nimllm {
@@ -130,97 +132,126 @@ __device__ __forceinline__ uint32_t score_key(float s) {
     return (x & 0x80000000u) ? ~x : (x | 0x80000000u);
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
+constexpr int kSelBins = 2048;
+constexpr int kSelKeys = 40960;        // keys that a block keeps in shared memory; a longer part is read again in every pass
 
-// One block per (sequence, KV head): the key of the last row that is kept by its score (radix select, 8 bits a pass), then
-// the kept rows in order.
+// A cluster of blocks per (sequence, KV head), each with a consecutive part of the rows: the key of the last row that is kept by its
+// score (radix select, digits of 11, 11 and 10 bits, histograms summed over the cluster's shared memory), then the kept rows in
+// order.  A warp has consecutive rows too, so that their places follow from one prefix over the warps.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p) {
-    __shared__ int s_hist[256];
-    __shared__ int s_digit, s_left;
-    __shared__ int s_eq[kSelThreads / 32], s_keep[kSelThreads / 32];
+    namespace cg = cooperative_groups;
+    extern __shared__ uint32_t s_key[];
+    __shared__ int s_hist[3][kSelBins];
+    __shared__ int s_warp[kSelWarps], s_digit, s_left;
+    __shared__ int2 s_cnt[kSelWarps];
+    __shared__ int2 s_total;
     launch_dependents();
     grid_dependency_wait();
-    const int pair = blockIdx.x, b = pair / p.Hkv;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    const int pair = blockIdx.x / parts, b = pair / p.Hkv;
     const int len = evict_len(p, b), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int32_t *kept = p.kept + (int64_t)pair * p.keep;
-    if (p.new_len && pair % p.Hkv == 0 && tid == 0) p.new_len[b] = min(len, p.keep);
-    if (len <= p.keep) {
-        for (int i = tid; i < p.keep; i += kSelThreads) kept[i] = i < len ? i : -1;
+    if (p.new_len && part == 0 && pair % p.Hkv == 0 && tid == 0) p.new_len[b] = min(len, p.keep);
+    if (len <= p.keep) {                                   // the same in every block of the cluster
+        for (int i = part * kSelThreads + tid; i < p.keep; i += parts * kSelThreads) kept[i] = i < len ? i : -1;
         return;
     }
     const float *score = p.score + (int64_t)pair * p.score_rows;
-    const int mid0 = p.n_sink, mid1 = len - p.n_recent;        // len > keep >= n_sink + n_recent
-    int left = p.keep - p.n_sink - p.n_recent;                 // rows still to be chosen among those at or below the prefix
+    const int mid0 = p.n_sink, mid1 = len - p.n_recent;    // len > keep >= n_sink + n_recent
+    // this block's rows: whole groups of 32 for every warp
+    const int per_warp = ((len + parts * kSelWarps - 1) / (parts * kSelWarps) + 31) / 32 * 32;
+    const int begin = part * kSelWarps * per_warp, rows = max(0, min(len - begin, kSelWarps * per_warp));
+    const bool in_smem = kSelWarps * per_warp <= kSelKeys;
+    if (in_smem)
+        for (int i = tid; i < rows; i += kSelThreads) s_key[i] = score_key(score[begin + i]);
+    for (int i = tid; i < 3 * kSelBins; i += kSelThreads) (&s_hist[0][0])[i] = 0;
+    __syncthreads();
+    auto key_of = [&](int i) { return in_smem ? s_key[i] : score_key(score[begin + i]); };
+    auto is_mid = [&](int i) { return begin + i >= mid0 && begin + i < mid1; };
+
+    const int wanted = p.keep - p.n_sink - p.n_recent;
+    int left = wanted;                                     // rows still to be chosen among those with the prefix
     uint32_t prefix = 0;
-    if (left > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s_hist[tid] = 0;
-            __syncthreads();
-            for (int r = mid0 + tid; r < mid1; r += kSelThreads) {
-                const uint32_t key = score_key(score[r]);
-                if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(key >> shift) & 255], 1);
+    if (wanted > 0) {
+#pragma unroll 1
+        for (int pass = 0; pass < 3; pass++) {
+            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11, above = shift + bits;
+            for (int i = tid; i < rows; i += kSelThreads) {
+                const uint32_t key = key_of(i);
+                if (is_mid(i) && (pass == 0 || (key >> above) == (prefix >> above))) atomicAdd(&s_hist[pass][(key >> shift) & ((1 << bits) - 1)], 1);
             }
-            __syncthreads();
-            if (warp == 0) {
-                // digits from the top: lane l holds 255 - 8l .. 248 - 8l
-                int c[8], sum = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) { c[j] = s_hist[255 - 8 * lane - j]; sum += c[j]; }
-                int incl = sum;
-#pragma unroll
-                for (int off = 1; off < 32; off <<= 1) {
-                    const int x = __shfl_up_sync(0xffffffffu, incl, off);
-                    if (lane >= off) incl += x;
-                }
-                int above = incl - sum;
-                if (above < left && incl >= left) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        if (above < left && above + c[j] >= left) { s_digit = 255 - 8 * lane - j; s_left = left - above; }
-                        above += c[j];
-                    }
-                }
+            cluster.sync();
+            // thread t has the digits 2047 - 2t and 2046 - 2t, highest first
+            int c0 = 0, c1 = 0;
+            for (int q = 0; q < parts; q++) {
+                const int *h = cluster.map_shared_rank(&s_hist[pass][0], q);
+                c0 += h[kSelBins - 1 - 2 * tid];
+                c1 += h[kSelBins - 2 - 2 * tid];
             }
+            int incl = c0 + c1;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += x;
+            }
+            if (lane == 31) s_warp[warp] = incl;
+            __syncthreads();
+            int before = incl - c0 - c1;
+            for (int w = 0; w < warp; w++) before += s_warp[w];
+            if (before < left && before + c0 >= left) { s_digit = kSelBins - 1 - 2 * tid; s_left = left - before; }
+            else if (before + c0 < left && before + c0 + c1 >= left) { s_digit = kSelBins - 2 - 2 * tid; s_left = left - before - c0; }
             __syncthreads();
             prefix |= (uint32_t)s_digit << shift;
             left = s_left;
-            __syncthreads();
         }
     }
-    // rows in order: 0.. n_sink, the middle rows above the last key or equal to it while any are left, the last n_recent
-    int eq_before = 0, kept_before = 0;
-    const bool none = p.keep == p.n_sink + p.n_recent;
-    for (int r0 = 0; r0 < len; r0 += kSelThreads) {
-        const int r = r0 + tid;
-        const bool mid = r >= mid0 && r < mid1;
-        const uint32_t key = mid ? score_key(score[r]) : 0u;
-        const bool eq = mid && !none && key == prefix;
-        const uint32_t eq_mask = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) s_eq[warp] = __popc(eq_mask);
-        __syncthreads();
-        int eq_rank = eq_before + __popc(eq_mask & ((1u << lane) - 1)), eq_all = 0;
-        for (int w = 0; w < kSelThreads / 32; w++) {
-            if (w < warp) eq_rank += s_eq[w];
-            eq_all += s_eq[w];
-        }
-        const bool take = r < len && (!mid || (!none && (key > prefix || (eq && eq_rank < left))));
-        const uint32_t mask = __ballot_sync(0xffffffffu, take);
-        if (lane == 0) s_keep[warp] = __popc(mask);
-        __syncthreads();
-        int at = kept_before + __popc(mask & ((1u << lane) - 1)), all = 0;
-        for (int w = 0; w < kSelThreads / 32; w++) {
-            if (w < warp) at += s_keep[w];
-            all += s_keep[w];
-        }
-        if (take) kept[at] = r;
-        eq_before += eq_all;
-        kept_before += all;
+    // kept: the rows in front and behind, the middle ones above the last key, and of those equal to it the first `left`
+    const int w0 = warp * per_warp, w1 = min(rows, w0 + per_warp);
+    int above = 0, equal = 0;
+    for (int i = w0 + lane; i < w1; i += 32) {
+        const uint32_t key = key_of(i);
+        const bool mid = is_mid(i);
+        above += !mid || (wanted > 0 && key > prefix);
+        equal += mid && wanted > 0 && key == prefix;
     }
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) s_cnt[warp] = make_int2(above, equal);
+    __syncthreads();
+    if (tid == 0) {
+        int2 t = make_int2(0, 0);
+        for (int w = 0; w < kSelWarps; w++) { t.x += s_cnt[w].x; t.y += s_cnt[w].y; }
+        s_total = t;
+    }
+    cluster.sync();
+    int above_before = 0, equal_before = 0;
+    for (int q = 0; q < part; q++) {
+        const int2 t = *cluster.map_shared_rank(&s_total, q);
+        above_before += t.x;
+        equal_before += t.y;
+    }
+    for (int w = 0; w < warp; w++) { above_before += s_cnt[w].x; equal_before += s_cnt[w].y; }
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t key = i < w1 ? key_of(i) : 0u;
+        const bool mid = is_mid(i);
+        const bool up = i < w1 && (!mid || (wanted > 0 && key > prefix)), eq = i < w1 && mid && wanted > 0 && key == prefix;
+        const uint32_t up_mask = __ballot_sync(0xffffffffu, up), eq_mask = __ballot_sync(0xffffffffu, eq), lower = (1u << lane) - 1;
+        const int eq_rank = equal_before + __popc(eq_mask & lower);
+        // in front of row i: all that are above, and the equal ones as far as they are kept
+        if (up || (eq && eq_rank < left)) kept[above_before + __popc(up_mask & lower) + min(eq_rank, left)] = begin + i;
+        above_before += __popc(up_mask);
+        equal_before += __popc(eq_mask);
+    }
+    cluster.sync();                                        // nobody leaves while its shared memory may still be read
 }
 
-constexpr int kMoveRows = 8;   // rows in flight per thread
+constexpr int kMoveThreads = 512, kMoveRows = 4;       // rows in flight per thread, twice
 
-__global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p) {
+// A block owns whole columns of one (sequence, KV head).  The loads of a batch are under way while the batch before is stored.
+__global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(EvictParams p) {
     launch_dependents();
     grid_dependency_wait();
     const int pair = blockIdx.x, b = pair / p.Hkv, kvh = pair - b * p.Hkv;
@@ -231,51 +262,69 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p) {
     if ((int)blockIdx.y == 2 * splits) {
         // the scores move with their rows; the rows to come start from nothing
         float *score = p.score + (int64_t)pair * p.score_rows;
-        for (int j0 = 0; j0 < p.keep; j0 += 256 * kMoveRows) {
-            float x[kMoveRows];
+        constexpr int kBatch = 8;
+        for (int j0 = 0; j0 < p.keep; j0 += kMoveThreads * kBatch) {
+            float x[kBatch];
 #pragma unroll
-            for (int u = 0; u < kMoveRows; u++) {
-                const int j = j0 + u * 256 + threadIdx.x;
+            for (int u = 0; u < kBatch; u++) {
+                const int j = j0 + u * kMoveThreads + threadIdx.x;
                 if (j < p.keep) x[u] = score[kept[j]];
             }
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < kMoveRows; u++) {
-                const int j = j0 + u * 256 + threadIdx.x;
+            for (int u = 0; u < kBatch; u++) {
+                const int j = j0 + u * kMoveThreads + threadIdx.x;
                 if (j < p.keep) score[j] = x[u];
             }
         }
         __syncthreads();
-        for (int r = p.keep + threadIdx.x; r < len; r += 256) score[r] = 0.f;
+        for (int r = p.keep + threadIdx.x; r < len; r += kMoveThreads) score[r] = 0.f;
         return;
     }
-    unsigned char *base = (int)blockIdx.y < splits ? p.k : p.v;
-    const int c = ((int)blockIdx.y % splits) * p.split16 + (int)threadIdx.x % p.split16;
-    const int rows_per_step = 256 / p.split16, row_in = (int)threadIdx.x / p.split16;
-    for (int j0 = 0; j0 < p.keep; j0 += rows_per_step * kMoveRows) {
-        uint4 x[kMoveRows];
-        int64_t to[kMoveRows];
+    unsigned char *base = ((int)blockIdx.y < splits ? p.k : p.v) + (((int)blockIdx.y % splits) * p.split16 + (int)threadIdx.x % p.split16) * 16;
+    const int step = kMoveThreads / p.split16, row_in = (int)threadIdx.x / p.split16, batch = step * kMoveRows;
+    const bool idle = row_in >= step;                      // threads that a piece of a row does not divide into
+    struct Rows { uint4 x[kMoveRows]; int64_t to[kMoveRows]; };
+    int next[kMoveRows];
+    auto fetch_index = [&](int j0) {
 #pragma unroll
         for (int u = 0; u < kMoveRows; u++) {
-            const int j = j0 + u * rows_per_step + row_in;
-            to[u] = -1;
-            if (j < p.keep) {
-                const int r = kept[j];
-                if (r != j) {
-                    const int64_t fro = cache_row(p.rows, b, kvh, r);
-                    to[u] = cache_row(p.rows, b, kvh, j);
-                    if (fro < 0) to[u] = -1;
-                    if (to[u] >= 0) {
-                        to[u] = to[u] * p.elem + c * 16;
-                        x[u] = *reinterpret_cast<const uint4 *>(base + fro * p.elem + c * 16);
-                    }
+            const int j = j0 + u * step + row_in;
+            next[u] = j < p.keep && !idle ? kept[j] : -1;
+        }
+    };
+    auto load = [&](Rows &r, int j0) {
+#pragma unroll
+        for (int u = 0; u < kMoveRows; u++) {
+            const int j = j0 + u * step + row_in;
+            r.to[u] = -1;
+            if (next[u] >= 0 && next[u] != j) {
+                const int64_t fro = cache_row(p.rows, b, kvh, next[u]), to = cache_row(p.rows, b, kvh, j);
+                if (fro >= 0 && to >= 0) {
+                    r.to[u] = to * p.elem;
+                    r.x[u] = __ldcs(reinterpret_cast<const uint4 *>(base + fro * p.elem));
                 }
             }
         }
-        __syncthreads();
+        fetch_index(j0 + batch);
+    };
+    auto store = [&](const Rows &r) {
 #pragma unroll
         for (int u = 0; u < kMoveRows; u++)
-            if (to[u] >= 0) *reinterpret_cast<uint4 *>(base + to[u]) = x[u];
+            if (r.to[u] >= 0) __stcs(reinterpret_cast<uint4 *>(base + r.to[u]), r.x[u]);
+    };
+    // a batch stores rows j .. j + batch - 1 only; the ones behind it have their sources at or behind j + batch, so they may be
+    // read before or after
+    Rows r0, r1;
+    fetch_index(0);
+    load(r0, 0);
+    for (int j0 = 0; j0 < p.keep; j0 += 2 * batch) {
+        load(r1, j0 + batch);
+        __syncthreads();
+        store(r0);
+        load(r0, j0 + 2 * batch);
+        __syncthreads();
+        store(r1);
     }
 }
 
@@ -302,12 +351,38 @@ int kv_evict(const char *who, const CacheRows &rows, void *k, void *v, int cache
     p.k = (unsigned char *)k; p.v = (unsigned char *)v; p.rows = rows; p.score = score; p.score_rows = score_rows; p.seq_len = seq_len;
     p.new_len = new_len == seq_len ? nullptr : new_len; p.kept = kept; p.max_len = max_len; p.keep = keep; p.n_sink = n_sink;
     p.n_recent = n_recent; p.B = batch; p.Hkv = n_kv_head; p.elem = elem; p.row16 = head_dim * elem / 16;
-    // 64-byte column pieces where the row divides into them: more blocks than (sequence, KV head) pairs
-    p.split16 = p.row16 % 4 == 0 ? 4 : (p.row16 % 2 == 0 ? 2 : 1);
+    // whole rows to a block while the (sequence, KV head) pairs fill the GPU, else column pieces of 64 bytes at least
+    const int64_t pairs = (int64_t)batch * n_kv_head;
+    p.split16 = p.row16;
+    while (p.split16 > 4 && p.split16 % 2 == 0 && 2 * pairs * (p.row16 / p.split16) < sm_count()) p.split16 /= 2;
+    if (p.split16 > kMoveThreads) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: head_dim %d", who, head_dim);
+    // blocks of a cluster: two on every SM, 2048 rows each at least
+    int parts = 1;
+    while (parts < 8 && pairs * parts < sm_count() && max_len >= parts * 4096) parts *= 2;
+    const size_t part_rows = (((size_t)max_len + parts * kSelWarps - 1) / (parts * kSelWarps) + 31) / 32 * 32 * kSelWarps;
+    const size_t smem = (part_rows <= kSelKeys ? part_rows : kSelKeys) * sizeof(uint32_t);
+    if (pairs * parts > 0x7fffffff) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: too many (sequence, KV head) pairs", who);
     cudaStream_t st = (cudaStream_t)stream;
-    cudaError_t e = launch_dependent(evict_select_kernel, dim3(batch * n_kv_head), kSelThreads, 0, st, p);
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
+        e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * (int)sizeof(uint32_t));
+        if (e == cudaSuccess && dev < 64) ready[dev] = true;
+    }
+    if (e == cudaSuccess) {
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(pairs * parts)); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+        cfg.attrs = attr; cfg.numAttrs = 2;
+        e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
+    }
     if (e == cudaSuccess)
-        e = launch_dependent(evict_move_kernel, dim3(batch * n_kv_head, 2 * (p.row16 / p.split16) + 1), 256, 0, st, p);
+        e = launch_dependent(evict_move_kernel, dim3((unsigned)pairs, 2 * (p.row16 / p.split16) + 1), kMoveThreads, 0, st, p);
     if (e == cudaSuccess && !p.new_len) e = launch_dependent(evict_lens_kernel, dim3((batch + 255) / 256), 256, 0, st, p, new_len);
     if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return NIMLLM_OK;

@@ -6,8 +6,8 @@
 // The other columns pass.  rope_append.cu ties the row of a token to its position; here both are given, because the tokens
 // of a drafted tree share positions and the rows of an evicted cache have left theirs.
 //
-// HBM-bound elementwise work.  A thread moves 2 vectors of V elements (16 bytes each where the head allows: V = 8 for bf16,
-// 4 for fp32; else 4), all of them rotated or all of them passed.
+// HBM-bound elementwise work.  A thread moves pairs of vectors of V elements (16 bytes each where the head allows: V = 8 for
+// bf16, 4 for fp32; else 4), all of them rotated or all of them passed.
 #include <math.h>
 
 #include "cache_rows.cuh"
@@ -29,19 +29,21 @@ struct RopeAtParams {
     float sign;
     int zero_padding;        // gradient: tokens without a position get 0 (the forward did not read them)
     int n_q, n_k, n_v;       // slots: query heads, K heads, V heads
+    int items, lanes, per_token;   // pairs of vectors of a head, threads of a token that have the same one, threads of a token
 };
 
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T *p, float *f) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 x = *reinterpret_cast<const float4 *>(p);
-        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
-    } else if constexpr (V == 8) {
-        Elem<__nv_bfloat16>::unpack(*reinterpret_cast<const uint4 *>(p), f);
-    } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(p);
-        f[0] = bf16lo(x.x); f[1] = bf16hi(x.x); f[2] = bf16lo(x.y); f[3] = bf16hi(x.y);
-    }
+    static_assert(sizeof(T) == 4 && V == 4, "table entries");
+    const float4 x = *reinterpret_cast<const float4 *>(p);
+    f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
 }
+template <typename T, int V> struct Unpack {
+    __device__ static void go(const uint4 &u, float *f) {
+        if constexpr (sizeof(T) == 4) Elem<float>::unpack(u, f);
+        else if constexpr (V == 8) Elem<__nv_bfloat16>::unpack(u, f);
+        else { f[0] = bf16lo(u.x); f[1] = bf16hi(u.x); f[2] = bf16lo(u.y); f[3] = bf16hi(u.y); }
+    }
+};
 template <typename T, int V> __device__ __forceinline__ void store_vec(T *p, const float *f) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -53,96 +55,122 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T *p, con
     }
 }
 
-// Work item = (token, slot, pair of vectors); slots 0.. are the query heads, then the K heads, then the V heads.
-template <typename ActT, typename CacheT, int V, bool INTERLEAVED>
+// Slots 0.. are the query heads, then the K heads, then the V heads.  A thread has one pair of vectors of a token and takes kHeads of
+// the token's slots, `lanes` apart: the token's row, position and table entries are fetched and the places worked out once for all of
+// them, and the loads of all of them are in flight together.
+template <typename ActT, typename CacheT, int V, bool INTERLEAVED, int HEADS>
 __global__ void __launch_bounds__(256) rope_at_kernel(RopeAtParams p) {
     launch_dependents();
     grid_dependency_wait();
-    const int items = p.D / (2 * V);
-    const int turned = p.rot / (2 * V);
-    const int half = p.rot / 2;
+    const int idx = blockIdx.x * 256 + threadIdx.x;        // < 2^31: checked on the host
+    const int token = idx / p.per_token;
+    if (token >= p.B * p.n) return;
+    const int in = idx - token * p.per_token;
+    const int first = in / p.items, item = in - first * p.items;
+    const int b = token / p.n, t = token - b * p.n;
     const int slots = p.n_q + p.n_k + p.n_v;
-    const int per_token = slots * items;
-    const int64_t total = (int64_t)p.B * p.n * per_token;
-    for (int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; idx < total; idx += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t token = idx / per_token;
-        const int in = (int)(idx - token * per_token);
-        const int slot = in / items, item = in - slot * items;
-        const int b = (int)(token / p.n), t = (int)(token - (int64_t)b * p.n);
-        const int row = (p.row0 ? p.row0[b] : p.first_row) + t;
-        const int pos = p.pos ? p.pos[token] : row;
-        const bool live = pos >= 0 && (p.rot == 0 || pos < p.table_rows);
 
+    const int row = (p.row0 ? p.row0[b] : p.first_row) + t;
+    const int pos = p.pos ? p.pos[token] : row;
+    const bool live = pos >= 0 && (p.rot == 0 || pos < p.table_rows);
+    // the first elements of the two vectors
+    const bool turned = item * 2 * V < p.rot;
+    const int half = p.rot / 2;
+    const int e0 = turned && !INTERLEAVED ? item * V : item * 2 * V;
+    const int e1 = turned && !INTERLEAVED ? e0 + half : e0 + V;
+
+    uint4 x0[HEADS], x1[HEADS];                            // V elements each, as they lie in memory
+    if (live) {
+#pragma unroll
+        for (int h = 0; h < HEADS; h++) {
+            const int slot = first + h * p.lanes;
+            if (slot < slots) {
+                const bool is_q = slot < p.n_q, is_v = slot >= p.n_q + p.n_k;
+                const int head = is_q ? slot : (is_v ? slot - p.n_q - p.n_k : slot - p.n_q);
+                const ActT *x = reinterpret_cast<const ActT *>(is_q ? p.q : (is_v ? p.v : p.k)) + ((int64_t)token * (is_q ? p.Hq : p.Hkv) + head) * p.D;
+                if constexpr (sizeof(ActT) * V == 16) {
+                    x0[h] = *reinterpret_cast<const uint4 *>(x + e0);
+                    x1[h] = *reinterpret_cast<const uint4 *>(x + e1);
+                } else {
+                    const uint2 y0 = *reinterpret_cast<const uint2 *>(x + e0), y1 = *reinterpret_cast<const uint2 *>(x + e1);
+                    x0[h] = make_uint4(y0.x, y0.y, 0, 0);
+                    x1[h] = make_uint4(y1.x, y1.y, 0, 0);
+                }
+            }
+        }
+    }
+    float c[V], s[V];
+    if (live && turned) {
+        const float *ct = p.cos_tab + (int64_t)pos * half + item * V, *st = p.sin_tab + (int64_t)pos * half + item * V;
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            load_vec<float, 4>(ct + i, c + i);
+            load_vec<float, 4>(st + i, s + i);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) s[i] *= p.sign;
+    }
+    const bool in_cache = p.k_cache && live && row >= 0 && row < p.rows.cap;
+#pragma unroll
+    for (int h = 0; h < HEADS; h++) {
+        const int slot = first + h * p.lanes;
+        if (slot >= slots) break;
         const bool is_q = slot < p.n_q, is_v = slot >= p.n_q + p.n_k;
         const int head = is_q ? slot : (is_v ? slot - p.n_q - p.n_k : slot - p.n_q);
-        const int64_t src = (token * (is_q ? p.Hq : p.Hkv) + head) * p.D;
         ActT *out = reinterpret_cast<ActT *>(is_q ? p.q_out : (is_v ? nullptr : p.k_out));
-        // the first elements of the two vectors
-        const bool turn = item < turned && !is_v;
-        int e0, e1;
-        if (item < turned) {
-            e0 = INTERLEAVED ? item * 2 * V : item * V;
-            e1 = INTERLEAVED ? e0 + V : e0 + half;
+        if (out) out += ((int64_t)token * (is_q ? p.Hq : p.Hkv) + head) * p.D;
+        float f0[V], f1[V];
+        if (live) {
+            Unpack<ActT, V>::go(x0[h], f0);
+            Unpack<ActT, V>::go(x1[h], f1);
+            if (turned && !is_v) {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    // pair i: (f0[i], f1[i]) in the half layout, two neighbours of the 2V elements in the interleaved one
+                    float &u = INTERLEAVED ? (2 * i < V ? f0[(2 * i) % V] : f1[(2 * i) % V]) : f0[i];
+                    float &w = INTERLEAVED ? (2 * i < V ? f0[(2 * i + 1) % V] : f1[(2 * i + 1) % V]) : f1[i];
+                    const float y0 = u * c[i] - w * s[i], y1 = u * s[i] + w * c[i];
+                    u = y0;
+                    w = y1;
+                }
+            }
         } else {
-            e0 = item * 2 * V;
-            e1 = e0 + V;
-        }
-        if (!live) {
-            if (p.zero_padding && out) {
-                float z[V];
+            if (!p.zero_padding) continue;
 #pragma unroll
-                for (int i = 0; i < V; i++) z[i] = 0.f;
-                store_vec<ActT, V>(out + src + e0, z);
-                store_vec<ActT, V>(out + src + e1, z);
-            }
-            continue;
-        }
-        const ActT *x = reinterpret_cast<const ActT *>(is_q ? p.q : (is_v ? p.v : p.k)) + src;
-        float x0[V], x1[V];
-        load_vec<ActT, V>(x + e0, x0);
-        load_vec<ActT, V>(x + e1, x1);
-        if (turn) {
-            const float *ct = p.cos_tab + (int64_t)pos * half, *st = p.sin_tab + (int64_t)pos * half;
-            float c[V], s[V];
-            const int f = item * V;
-#pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                load_vec<float, 4>(ct + f + i, c + i);
-                load_vec<float, 4>(st + f + i, s + i);
-            }
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float sn = p.sign * s[i];
-                // pair i: (x0[i], x1[i]) in the half layout, two neighbours of the 2V elements in the interleaved one
-                float &a = INTERLEAVED ? (2 * i < V ? x0[(2 * i) % V] : x1[(2 * i) % V]) : x0[i];
-                float &d = INTERLEAVED ? (2 * i < V ? x0[(2 * i + 1) % V] : x1[(2 * i + 1) % V]) : x1[i];
-                const float y0 = a * c[i] - d * sn, y1 = a * sn + d * c[i];
-                a = y0;
-                d = y1;
-            }
+            for (int i = 0; i < V; i++) f0[i] = f1[i] = 0.f;
         }
         if (out) {
-            store_vec<ActT, V>(out + src + e0, x0);
-            store_vec<ActT, V>(out + src + e1, x1);
+            store_vec<ActT, V>(out + e0, f0);
+            store_vec<ActT, V>(out + e1, f1);
         }
-        if (!is_q && p.k_cache && row >= 0 && row < p.rows.cap) {
+        if (!is_q && in_cache) {
             const int64_t at = cache_row(p.rows, b, head, row);
             if (at >= 0) {
                 CacheT *dst = reinterpret_cast<CacheT *>(is_v ? p.v_cache : p.k_cache) + at;
-                store_vec<CacheT, V>(dst + e0, x0);
-                store_vec<CacheT, V>(dst + e1, x1);
+                store_vec<CacheT, V>(dst + e0, f0);
+                store_vec<CacheT, V>(dst + e1, f1);
             }
         }
     }
 }
 
+template <typename ActT, typename CacheT, int V, int HEADS>
+cudaError_t launch_heads(RopeAtParams p, int layout, cudaStream_t st) {
+    const int slots = p.n_q + p.n_k + p.n_v;
+    p.items = p.D / (2 * V);
+    p.lanes = (slots + HEADS - 1) / HEADS;
+    p.per_token = p.lanes * p.items;
+    const int64_t threads = (int64_t)p.B * p.n * p.per_token;
+    if (threads > 0x7fffff00) return cudaErrorInvalidConfiguration;
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    return layout == NIMLLM_ROPE_INTERLEAVED ? launch_dependent(rope_at_kernel<ActT, CacheT, V, true, HEADS>, grid, 256, 0, st, p)
+                                             : launch_dependent(rope_at_kernel<ActT, CacheT, V, false, HEADS>, grid, 256, 0, st, p);
+}
 template <typename ActT, typename CacheT, int V>
 cudaError_t launch_v(const RopeAtParams &p, int layout, cudaStream_t st) {
-    const int64_t total = (int64_t)p.B * p.n * (p.n_q + p.n_k + p.n_v) * (p.D / (2 * V));
-    const int64_t blocks = (total + 255) / 256, cap = (int64_t)sm_count() * 32;
-    const dim3 grid((unsigned)(blocks < cap ? blocks : cap));
-    return layout == NIMLLM_ROPE_INTERLEAVED ? launch_dependent(rope_at_kernel<ActT, CacheT, V, true>, grid, 256, 0, st, p)
-                                             : launch_dependent(rope_at_kernel<ActT, CacheT, V, false>, grid, 256, 0, st, p);
+    // four heads a thread once that still leaves every SM full of threads
+    const int64_t threads = (int64_t)p.B * p.n * (p.n_q + p.n_k + p.n_v) * (p.D / (2 * V));
+    return threads >= (int64_t)sm_count() * 2048 * 4 ? launch_heads<ActT, CacheT, V, 4>(p, layout, st) : launch_heads<ActT, CacheT, V, 1>(p, layout, st);
 }
 
 int launch_rope_at(const char *who, const RopeAtParams &p, int layout, int act_dtype, int cache_dtype, cudaStream_t st) {
@@ -161,6 +189,7 @@ int launch_rope_at(const char *who, const RopeAtParams &p, int layout, int act_d
 
 int check_rotation(const char *who, int act_dtype, const float *cos_tab, const float *sin_tab, int rot_dim, int layout, int table_rows,
                    int batch, int n, int n_head, int n_kv_head, int head_dim) {
+    if ((int64_t)batch * n > 0x7fffffff) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: %d x %d tokens", who, batch, n);
     if (batch < 0 || n < 0 || n_head < 0 || n_kv_head < 0 || head_dim <= 0 || head_dim % 8 != 0)
         return fail(NIMLLM_ERR_ARG, "%s: bad shape B=%d n=%d Hq=%d Hkv=%d D=%d", who, batch, n, n_head, n_kv_head, head_dim);
     if (!dtype_ok(act_dtype)) return fail(NIMLLM_ERR_ARG, "%s: unknown dtype", who);
