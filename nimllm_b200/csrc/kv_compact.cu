@@ -198,8 +198,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
             }
             if (lane == 31) s_warp[warp] = incl;
             __syncthreads();
-            int before = incl - c0 - c1;
-            for (int w = 0; w < warp; w++) before += s_warp[w];
+            int before = incl - c0 - c1 + __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane] : 0);
             if (before < left && before + c0 >= left) { s_digit = kSelBins - 1 - 2 * tid; s_left = left - before; }
             else if (before + c0 < left && before + c0 + c1 >= left) { s_digit = kSelBins - 2 - 2 * tid; s_left = left - before - c0; }
             __syncthreads();
@@ -220,10 +219,10 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) s_cnt[warp] = make_int2(above, equal);
     __syncthreads();
-    if (tid == 0) {
-        int2 t = make_int2(0, 0);
-        for (int w = 0; w < kSelWarps; w++) { t.x += s_cnt[w].x; t.y += s_cnt[w].y; }
-        s_total = t;
+    const int2 mine = s_cnt[lane];
+    if (warp == 0) {
+        const int x = __reduce_add_sync(0xffffffffu, mine.x), y = __reduce_add_sync(0xffffffffu, mine.y);
+        if (lane == 0) s_total = make_int2(x, y);
     }
     cluster.sync();
     int above_before = 0, equal_before = 0;
@@ -232,7 +231,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
         above_before += t.x;
         equal_before += t.y;
     }
-    for (int w = 0; w < warp; w++) { above_before += s_cnt[w].x; equal_before += s_cnt[w].y; }
+    above_before += __reduce_add_sync(0xffffffffu, lane < warp ? mine.x : 0);
+    equal_before += __reduce_add_sync(0xffffffffu, lane < warp ? mine.y : 0);
     for (int i0 = w0; i0 < w1; i0 += 32) {
         const int i = i0 + lane;
         const uint32_t key = i < w1 ? key_of(i) : 0u;
@@ -248,13 +248,16 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
     cluster.sync();                                        // nobody leaves while its shared memory may still be read
 }
 
-constexpr int kMoveThreads = 512, kMoveRows = 4;       // rows in flight per thread, twice
+constexpr int kMoveThreads = 512, kMoveRows = 4, kMoveStages = 3;      // rows of a thread in a batch, batches under way
+constexpr int kMoveSmem = kMoveStages * kMoveRows * kMoveThreads * 16;
 
-// A block owns whole columns of one (sequence, KV head).  The loads of a batch are under way while the batch before is stored.
+// A block owns whole columns of one (sequence, KV head).  Batches are fetched with cp.async into shared memory that only the fetching
+// thread reads again, two batches ahead of the one that is stored.
 __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(EvictParams p) {
+    extern __shared__ uint4 s_move[];
     launch_dependents();
     grid_dependency_wait();
-    const int pair = blockIdx.x, b = pair / p.Hkv, kvh = pair - b * p.Hkv;
+    const int pair = blockIdx.x, b = pair / p.Hkv, kvh = pair - b * p.Hkv, tid = threadIdx.x;
     const int len = evict_len(p, b);
     if (len <= p.keep) return;
     const int32_t *kept = p.kept + (int64_t)pair * p.keep;
@@ -267,25 +270,33 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(EvictParams
             float x[kBatch];
 #pragma unroll
             for (int u = 0; u < kBatch; u++) {
-                const int j = j0 + u * kMoveThreads + threadIdx.x;
+                const int j = j0 + u * kMoveThreads + tid;
                 if (j < p.keep) x[u] = score[kept[j]];
             }
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < kBatch; u++) {
-                const int j = j0 + u * kMoveThreads + threadIdx.x;
+                const int j = j0 + u * kMoveThreads + tid;
                 if (j < p.keep) score[j] = x[u];
             }
         }
         __syncthreads();
-        for (int r = p.keep + threadIdx.x; r < len; r += kMoveThreads) score[r] = 0.f;
+        for (int r = p.keep + tid; r < len; r += kMoveThreads) score[r] = 0.f;
         return;
     }
-    unsigned char *base = ((int)blockIdx.y < splits ? p.k : p.v) + (((int)blockIdx.y % splits) * p.split16 + (int)threadIdx.x % p.split16) * 16;
-    const int step = kMoveThreads / p.split16, row_in = (int)threadIdx.x / p.split16, batch = step * kMoveRows;
+    const int step = kMoveThreads / p.split16, row_in = tid / p.split16, batch = step * kMoveRows;
     const bool idle = row_in >= step;                      // threads that a piece of a row does not divide into
-    struct Rows { uint4 x[kMoveRows]; int64_t to[kMoveRows]; };
-    int next[kMoveRows];
+    unsigned char *base = ((int)blockIdx.y < splits ? p.k : p.v) + (((int)blockIdx.y % splits) * p.split16 + tid % p.split16) * 16;
+    const bool paged = p.rows.table != nullptr;
+    const int row_bytes = p.row16 * 16;
+    if (!paged) base += cache_row(p.rows, b, kvh, 0) * p.elem;
+    auto row_at = [&](int r) -> int64_t {                  // bytes from base; < 0: no page
+        if (!paged) return (int64_t)r * row_bytes;
+        const int64_t at = cache_row(p.rows, b, kvh, r);
+        return at < 0 ? -1 : at * p.elem;
+    };
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_move) + tid * 16;
+    int next[kMoveRows];                                   // the sources of the batch that is fetched next
     auto fetch_index = [&](int j0) {
 #pragma unroll
         for (int u = 0; u < kMoveRows; u++) {
@@ -293,39 +304,42 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(EvictParams
             next[u] = j < p.keep && !idle ? kept[j] : -1;
         }
     };
-    auto load = [&](Rows &r, int j0) {
+    uint32_t moves[kMoveStages];                           // per stage: the rows that move, one bit each
+    auto fetch = [&](int stage, int j0) {
+        uint32_t m = 0;
 #pragma unroll
         for (int u = 0; u < kMoveRows; u++) {
             const int j = j0 + u * step + row_in;
-            r.to[u] = -1;
             if (next[u] >= 0 && next[u] != j) {
-                const int64_t fro = cache_row(p.rows, b, kvh, next[u]), to = cache_row(p.rows, b, kvh, j);
-                if (fro >= 0 && to >= 0) {
-                    r.to[u] = to * p.elem;
-                    r.x[u] = __ldcs(reinterpret_cast<const uint4 *>(base + fro * p.elem));
+                const int64_t fro = row_at(next[u]);
+                if (fro >= 0 && (!paged || row_at(j) >= 0)) {
+                    m |= 1u << u;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (stage * kMoveRows + u) * (kMoveThreads * 16)), "l"(base + fro) : "memory");
                 }
             }
         }
+        moves[stage] = m;
+        asm volatile("cp.async.commit_group;" ::: "memory");
         fetch_index(j0 + batch);
     };
-    auto store = [&](const Rows &r) {
-#pragma unroll
-        for (int u = 0; u < kMoveRows; u++)
-            if (r.to[u] >= 0) __stcs(reinterpret_cast<uint4 *>(base + r.to[u]), r.x[u]);
-    };
-    // a batch stores rows j .. j + batch - 1 only; the ones behind it have their sources at or behind j + batch, so they may be
-    // read before or after
-    Rows r0, r1;
+    // A batch stores rows j .. j + batch - 1 only, behind the barrier that says that everybody has fetched it; the batches behind it have
+    // their sources at or behind j + batch and may be fetched before or after.
     fetch_index(0);
-    load(r0, 0);
-    for (int j0 = 0; j0 < p.keep; j0 += 2 * batch) {
-        load(r1, j0 + batch);
-        __syncthreads();
-        store(r0);
-        load(r0, j0 + 2 * batch);
-        __syncthreads();
-        store(r1);
+#pragma unroll
+    for (int t = 0; t < kMoveStages - 1; t++) fetch(t, t * batch);
+    for (int j0 = 0; j0 < p.keep; j0 += kMoveStages * batch) {
+#pragma unroll
+        for (int t = 0; t < kMoveStages; t++) {
+            fetch((t + kMoveStages - 1) % kMoveStages, j0 + (t + kMoveStages - 1) * batch);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kMoveStages - 1) : "memory");
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < kMoveRows; u++)
+                if ((moves[t] >> u) & 1)
+                    __stcs(reinterpret_cast<uint4 *>(base + row_at(j0 + t * batch + u * step + row_in)), s_move[(t * kMoveRows + u) * kMoveThreads + tid]);
+        }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(256) evict_lens_kernel(EvictParams p, int32_t *new_len) {
@@ -356,9 +370,9 @@ int kv_evict(const char *who, const CacheRows &rows, void *k, void *v, int cache
     p.split16 = p.row16;
     while (p.split16 > 4 && p.split16 % 2 == 0 && 2 * pairs * (p.row16 / p.split16) < sm_count()) p.split16 /= 2;
     if (p.split16 > kMoveThreads) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: head_dim %d", who, head_dim);
-    // blocks of a cluster: two on every SM, 2048 rows each at least
+    // blocks of a cluster: as many as the SMs hold at once, 2048 rows each at least
     int parts = 1;
-    while (parts < 8 && pairs * parts < sm_count() && max_len >= parts * 4096) parts *= 2;
+    while (parts < 8 && 2 * pairs * parts <= sm_count() && max_len >= parts * 4096) parts *= 2;
     const size_t part_rows = (((size_t)max_len + parts * kSelWarps - 1) / (parts * kSelWarps) + 31) / 32 * 32 * kSelWarps;
     const size_t smem = (part_rows <= kSelKeys ? part_rows : kSelKeys) * sizeof(uint32_t);
     if (pairs * parts > 0x7fffffff) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: too many (sequence, KV head) pairs", who);
@@ -368,6 +382,7 @@ int kv_evict(const char *who, const CacheRows &rows, void *k, void *v, int cache
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
         e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * (int)sizeof(uint32_t));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoveSmem);
         if (e == cudaSuccess && dev < 64) ready[dev] = true;
     }
     if (e == cudaSuccess) {
@@ -382,7 +397,7 @@ int kv_evict(const char *who, const CacheRows &rows, void *k, void *v, int cache
         e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
     }
     if (e == cudaSuccess)
-        e = launch_dependent(evict_move_kernel, dim3((unsigned)pairs, 2 * (p.row16 / p.split16) + 1), kMoveThreads, 0, st, p);
+        e = launch_dependent(evict_move_kernel, dim3((unsigned)pairs, 2 * (p.row16 / p.split16) + 1), kMoveThreads, kMoveSmem, st, p);
     if (e == cudaSuccess && !p.new_len) e = launch_dependent(evict_lens_kernel, dim3((batch + 255) / 256), 256, 0, st, p, new_len);
     if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return NIMLLM_OK;

@@ -184,9 +184,17 @@ __global__ void __launch_bounds__(kFinishThreads, 5) tree_finish_kernel(TreePara
 #pragma unroll
     for (int g = 0; g < kAhead; g++) ahead[g] = in_raw && g < p.G ? __ldcs(reinterpret_cast<const float4 *>(raw + g * p.raw_ld)) : make_float4(0.f, 0.f, 0.f, 0.f);
     float *s = p.score + ((int64_t)b * p.Hkv + kvh) * p.score_rows + row;
-    float old[4];
+    const bool vec = row + 4 <= p.max_len && !((uintptr_t)s & 15);
+    float old[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.decay != 0.f) {
+        if (vec) {
+            const float4 o = *reinterpret_cast<const float4 *>(s);
+            old[0] = o.x; old[1] = o.y; old[2] = o.z; old[3] = o.w;
+        } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++) old[j] = p.decay != 0.f && row + j < p.max_len ? s[j] : 0.f;
+            for (int j = 0; j < 4; j++) old[j] = row + j < p.max_len ? s[j] : 0.f;
+        }
+    }
     float2 st = make_float2(0.f, 0.f);
     if ((int)threadIdx.x < min(256, p.G)) st = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + threadIdx.x));
     const int len = tree_committed(p, b);
@@ -222,8 +230,14 @@ __global__ void __launch_bounds__(kFinishThreads, 5) tree_finish_kernel(TreePara
     // the four rows lie in one page (page_rows >= 32); without a page they have no raw score
     if (row >= len || (p.rows.table && cache_row(p.rows, b, kvh, row) < 0)) return;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (row + j < len) s[j] = (p.decay == 0.f ? 0.f : p.decay * old[j]) + sum[j];
+    for (int j = 0; j < 4; j++) sum[j] += p.decay == 0.f ? 0.f : p.decay * old[j];
+    if (vec && row + 4 <= len) {
+        *reinterpret_cast<float4 *>(s) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (row + j < len) s[j] = sum[j];
+    }
 }
 
 template <int D> inline cudaError_t launch_finish(const TreeParams &p, FinishArgs &f, cudaStream_t st) {
