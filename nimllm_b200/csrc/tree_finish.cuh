@@ -9,7 +9,7 @@
 namespace nimllm {
 namespace treetc {
 
-constexpr int kFinishThreads = 256, kScoreRows = 4 * kFinishThreads;
+constexpr int kFinishThreads = 256, kScoreRows = 4096;
 constexpr int kMaxPieces = 180;        // 32 rows of them in 48 KB
 
 // The pieces of a query row.  Tensor-core kernels: records of consecutive CTAs (tree_tc.cuh); CUDA-core kernel: one record per chunk of
@@ -120,8 +120,8 @@ __device__ __forceinline__ void join_rows(const TreeParams &p, const Pieces &x, 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kFinishThreads, 5) tree_finish_kernel(TreeParams p, FinishArgs f) {
-    extern __shared__ float2 s_dyn[];                      // join: kJoinRows x pieces; score: 256 heads
+__global__ void __launch_bounds__(kFinishThreads, 4) tree_finish_kernel(TreeParams p, FinishArgs f) {
+    extern __shared__ float2 s_dyn[];                      // join: kJoinRows x pieces; score: the G heads
     float2 *s_stat = s_dyn;
     launch_dependents();
     grid_dependency_wait();
@@ -171,72 +171,76 @@ __global__ void __launch_bounds__(kFinishThreads, 5) tree_finish_kernel(TreePara
         return;
     }
     x -= f.n_zero;
-    // score[r] = decay * score[r] + sum over the G heads of exp2(raw - m) / l, four rows a thread.  What a block reads first -- length,
-    // statistics, raw scores, old scores -- has addresses that depend on nothing, so that its loads wait for memory together.
+    // score[r] = decay * score[r] + sum over the G heads of exp2(raw - m) / l: a block has up to 4096 rows of a pair, four a thread at a
+    // time.  What it reads first -- length, statistics, raw scores, old scores -- has addresses that depend on nothing, so that its
+    // loads wait for memory together, and the next rows' are under way while these are worked on.
     const int blocks = (p.max_len + kScoreRows - 1) / kScoreRows;
     const int pair = x / blocks, b = pair / p.Hkv, kvh = pair - b * p.Hkv;
-    const int r0 = (x - pair * blocks) * kScoreRows, row = r0 + threadIdx.x * 4;
+    const int r0 = (x - pair * blocks) * kScoreRows;
     const int64_t h0 = (int64_t)b * p.Hq + kvh * p.G;
-    const float *raw = p.raw + h0 * p.raw_ld + row;
-    constexpr int kAhead = 4;
-    float4 ahead[kAhead];
-    const bool in_raw = row < p.max_len;                   // the workspace holds whole rows of scores, whatever the length
+    const float *raw = p.raw + h0 * p.raw_ld;
+    float *score = p.score + (int64_t)pair * p.score_rows;
+    const bool vec = !((uintptr_t)score & 15);
+    constexpr int kAhead = 4;                              // heads whose raw scores are fetched ahead
+    struct Ahead { float4 raw[kAhead], old; };
+    auto fetch = [&](Ahead &a, int row) {                  // the workspace holds whole rows of raw scores, whatever the length
 #pragma unroll
-    for (int g = 0; g < kAhead; g++) ahead[g] = in_raw && g < p.G ? __ldcs(reinterpret_cast<const float4 *>(raw + g * p.raw_ld)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    float *s = p.score + ((int64_t)b * p.Hkv + kvh) * p.score_rows + row;
-    const bool vec = row + 4 <= p.max_len && !((uintptr_t)s & 15);
-    float old[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.decay != 0.f) {
-        if (vec) {
-            const float4 o = *reinterpret_cast<const float4 *>(s);
-            old[0] = o.x; old[1] = o.y; old[2] = o.z; old[3] = o.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) old[j] = row + j < p.max_len ? s[j] : 0.f;
+        for (int g = 0; g < kAhead; g++) a.raw[g] = row < p.max_len && g < p.G ? __ldcs(reinterpret_cast<const float4 *>(raw + g * p.raw_ld + row)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        a.old = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.decay != 0.f) {
+            if (vec && row + 4 <= p.max_len) {
+                a.old = *reinterpret_cast<const float4 *>(score + row);
+            } else {
+                if (row < p.max_len) a.old.x = score[row];
+                if (row + 1 < p.max_len) a.old.y = score[row + 1];
+                if (row + 2 < p.max_len) a.old.z = score[row + 2];
+                if (row + 3 < p.max_len) a.old.w = score[row + 3];
+            }
         }
-    }
-    float2 st = make_float2(0.f, 0.f);
-    if ((int)threadIdx.x < min(256, p.G)) st = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + threadIdx.x));
+    };
+    int row = r0 + threadIdx.x * 4;
+    Ahead now;
+    fetch(now, row);
+    for (int g = threadIdx.x; g < p.G; g += kFinishThreads) s_stat[g] = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + g));
     const int len = tree_committed(p, b);
     if (r0 >= len) return;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int g0 = 0; g0 < p.G; g0 += 256) {
-        const int n = min(256, p.G - g0);
-        if (g0) {
-            __syncthreads();
-            if ((int)threadIdx.x < n) st = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + g0 + threadIdx.x));
+    __syncthreads();
+    // a negative sum marks a row that was cut: its pieces are joined here (all heads of a pair are cut alike)
+    if (s_stat[0].y < 0.f) {
+        __syncthreads();
+        for (int g = warp; g < p.G; g += kFinishThreads / 32) {
+            const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g, len, p.G) : chunk_pieces<D>(p, h0 + g, len);
+            float M, L;
+            pieces_stats<D>(pc, lane, M, L);
+            if (lane == 0) s_stat[g] = make_float2(M * kLog2e, L > 0.f ? 1.f / L : 0.f);
         }
-        if ((int)threadIdx.x < n) s_stat[threadIdx.x] = st;
-        // a negative sum marks a row that was cut: its pieces are joined here
-        if (__syncthreads_or((int)threadIdx.x < n && st.y < 0.f)) {
-            for (int g = warp; g < n; g += 8) {
-                const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g0 + g, len, p.G) : chunk_pieces<D>(p, h0 + g0 + g, len);
-                float M, L;
-                pieces_stats<D>(pc, lane, M, L);
-                if (lane == 0) s_stat[g] = make_float2(M * kLog2e, L > 0.f ? 1.f / L : 0.f);
-            }
-            __syncthreads();
-        }
-        if (row < len) {
-#pragma unroll 4
-            for (int g = 0; g < n; g++) {
-                const float4 v = g0 == 0 && g < kAhead ? ahead[g & (kAhead - 1)] : *reinterpret_cast<const float4 *>(raw + (g0 + g) * p.raw_ld);
-                const float2 t = s_stat[g];
-                sum[0] += ex2(v.x - t.x) * t.y; sum[1] += ex2(v.y - t.x) * t.y;
-                sum[2] += ex2(v.z - t.x) * t.y; sum[3] += ex2(v.w - t.x) * t.y;
-            }
-        }
+        __syncthreads();
     }
-    // the four rows lie in one page (page_rows >= 32); without a page they have no raw score
-    if (row >= len || (p.rows.table && cache_row(p.rows, b, kvh, row) < 0)) return;
+    for (; row < min(len, r0 + kScoreRows); row += 4 * kFinishThreads) {
+        Ahead next;
+        if (row + 4 * kFinishThreads < min(len, r0 + kScoreRows)) fetch(next, row + 4 * kFinishThreads);
+        float sum[4] = {p.decay * now.old.x, p.decay * now.old.y, p.decay * now.old.z, p.decay * now.old.w};
+        auto head = [&](const float4 &v, int g) {
+            const float2 t = s_stat[g];
+            sum[0] += ex2(v.x - t.x) * t.y; sum[1] += ex2(v.y - t.x) * t.y;
+            sum[2] += ex2(v.z - t.x) * t.y; sum[3] += ex2(v.w - t.x) * t.y;
+        };
 #pragma unroll
-    for (int j = 0; j < 4; j++) sum[j] += p.decay == 0.f ? 0.f : p.decay * old[j];
-    if (vec && row + 4 <= len) {
-        *reinterpret_cast<float4 *>(s) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-    } else {
+        for (int g = 0; g < kAhead; g++)
+            if (g < p.G) head(now.raw[g], g);
+#pragma unroll 4
+        for (int g = kAhead; g < p.G; g++) head(*reinterpret_cast<const float4 *>(raw + g * p.raw_ld + row), g);
+        // the four rows lie in one page (page_rows >= 32); without a page they have no raw score
+        if (!p.rows.table || cache_row(p.rows, b, kvh, row) >= 0) {
+            if (vec && row + 4 <= len) {
+                *reinterpret_cast<float4 *>(score + row) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+            } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (row + j < len) s[j] = sum[j];
+                for (int j = 0; j < 4; j++)
+                    if (row + j < len) score[row + j] = sum[j];
+            }
+        }
+        now = next;
     }
 }
 
@@ -255,7 +259,7 @@ template <int D> inline cudaError_t launch_finish(const TreeParams &p, FinishArg
     if (blocks == 0) return cudaSuccess;
     if (blocks > 0x7fffffff || pieces > kMaxPieces) return cudaErrorInvalidConfiguration;
     size_t smem = f.n_join ? kJoinRows * pieces * sizeof(float2) : 0;
-    if (smem < 256 * sizeof(float2)) smem = 256 * sizeof(float2);
+    if (p.score && smem < p.G * sizeof(float2)) smem = p.G * sizeof(float2);
     return launch_dependent(tree_finish_kernel<D>, dim3((unsigned)blocks), kFinishThreads, smem, st, p, f);
 }
 
