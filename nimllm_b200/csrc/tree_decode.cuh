@@ -1,4 +1,4 @@
-// tree_decode.cuh -- what the kernels of tree_decode.cu and tree_wide_tc.cu share.
+// tree_decode.cuh -- what the kernels of tree and scored decode share.
 #pragma once
 #include "cache_rows.cuh"
 
@@ -52,8 +52,10 @@ __device__ __forceinline__ int64_t tree_out_row(const TreeParams &p, int b, int 
     return ((int64_t)b * p.n + i) * p.Hq + kvh * p.G + (qr - i * p.G);
 }
 
-// the tensor-core kernel for bf16 caches (tree_wide_tc.cu)
+// the kernels for bf16 caches (tree_wide_tc.cu, tree_narrow_tc.cu) and for fp32 caches (tree_f32.cu)
 size_t tree_tc_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim);
+size_t tree_f32_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, int max_total);
+int launch_tree_f32(const char *who, TreeParams &p, int head_dim, int max_total, void *workspace, cudaStream_t st);
 int launch_tree_tc(const char *who, TreeParams &p, int head_dim, void *workspace, cudaStream_t st);
 
 }  // namespace nimllm

@@ -139,14 +139,14 @@ __global__ void __launch_bounds__(kFinishThreads, 4) tree_finish_kernel(TreePara
             return;
         }
         // the pair whose first cut is where CTA w begins; `per` blocks share its rows
-        const int per = f.rpt / kJoinRows, w = x / per + 1, first = (x % per) * kJoinRows;
+        const int per = f.rpt > kJoinRows ? f.rpt / kJoinRows : 1, w = x / per + 1, first = (x % per) * kJoinRows;
         const int64_t T = f.tc.cum[p.B];
         const int4 at = f.tc.starts[w];                    // sequence, KV head and q tile, tile (not written past the last worker)
         const int wa = (int)(T < f.workers ? T : f.workers);
         if (w >= wa || at.z == 0 || owner_of(first_unit(w, T, wa) - at.z, T, wa) != w - 1) return;
         const int len = tree_committed(p, at.x), total = len + tree_drafts(p, at.x, len), R = tree_tokens(p, at.x) * p.G;
         const int q_tiles = (R + f.rpt - 1) / f.rpt, kvh = at.y / q_tiles, q0 = (at.y - kvh * q_tiles) * f.rpt + first;
-        const int rows = min(kJoinRows, R - q0);
+        const int rows = min(min(kJoinRows, f.rpt), R - q0);
         if (rows > 0)
             join_rows<D>(p, tc_pieces<D>(p, f, at.x, kvh, q0, total, R), rows, [&](int r) { return tree_out_row(p, at.x, kvh, q0 + r); }, s_dyn);
         return;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kFinishThreads, 4) tree_finish_kernel(TreePara
 template <int D> inline cudaError_t launch_finish(const TreeParams &p, FinishArgs &f, cudaStream_t st) {
     size_t pieces;
     if (f.workers) {
-        f.n_join = (f.workers - 1) * (f.rpt / kJoinRows);
+        f.n_join = (f.workers - 1) * (f.rpt > kJoinRows ? f.rpt / kJoinRows : 1);
         f.n_zero = (p.B + 31) / 32;
         pieces = f.workers;
     } else {
