@@ -245,45 +245,45 @@ def _layout(name):
         raise _lib.NimllmAttnError(f"unknown layout {name!r}: 'half' and 'interleaved' are built") from None
 
 
-def _args(device, dtypes, *tensors):
-    """Data pointers of contiguous tensors on one device, each of its dtype (None: any), which is the current one.
-    None stays None."""
+def _refuse(t, dtype, index):
+    _ptr(t)
+    if t.get_device() != index:
+        raise _lib.NimllmAttnError(f"tensors on cuda:{t.get_device()} and on cuda:{index}")
+    raise _lib.NimllmAttnError(f"{dtype} tensor expected, got {t.dtype}")
+
+
+def _args(index, dtypes, tensors):
+    """Data pointers of contiguous tensors on device `index`, each of its dtype (None: any).  None stays None."""
     ptrs = []
     for t, dt in zip(tensors, dtypes):
         if t is None:
             ptrs.append(None)
-            continue
-        if t.device != device:
-            raise _lib.NimllmAttnError(f"tensors on {t.device} and on {device}")
-        if dt is not None and t.dtype != dt:
-            raise _lib.NimllmAttnError(f"{dt} tensor expected, got {t.dtype}")
-        ptrs.append(_ptr(t))
+        else:
+            if t.get_device() != index or (dt is not None and t.dtype is not dt) or not t.is_contiguous():
+                _refuse(t, dt, index)
+            ptrs.append(t.data_ptr())
     return ptrs
 
 
-def _sizes(**named):
-    """Every tensor holds at least the elements that its shape arguments say."""
-    for name, (t, least) in named.items():
-        if t is not None and t.numel() < least:
-            raise _lib.NimllmAttnError(f"{name} holds {t.numel()} elements, {least} are needed")
+def _small(name, t, least):
+    raise _lib.NimllmAttnError(f"{name} holds {t.numel()} elements, {least} are needed")
 
 
-def _block_sizes(k_cache, v_cache, kv_off, batch, n_kv_head, head_dim, seq_stride, head_stride, max_seq, layers=0, layer_stride=0):
-    """Without kv_off the blocks' ends are known: they have to lie in the tensors."""
-    if kv_off is not None or max_seq <= 0:
-        return
-    end = max(layers - 1, 0) * layer_stride + (batch - 1) * seq_stride + (n_kv_head - 1) * head_stride + max_seq * head_dim
-    _sizes(k_cache=(k_cache, end), v_cache=(v_cache, end))
+def _block_end(batch, n_kv_head, head_dim, seq_stride, head_stride, max_seq, layers=0, layer_stride=0):
+    """Elements that the blocks of a contiguous cache without kv_off reach over."""
+    return (layers - 1 if layers > 1 else 0) * layer_stride + (batch - 1) * seq_stride + (n_kv_head - 1) * head_stride + max_seq * head_dim
 
 
-def _on(device):
-    """The context in which a call for tensors of `device` launches."""
-    if device.type != "cuda":
-        raise _lib.NimllmAttnError("device tensor expected (there is no CPU path)")
-    return _same if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _check_blocks(k_cache, v_cache, end):
+    if k_cache.numel() < end:
+        _small("k_cache", k_cache, end)
+    if v_cache.numel() < end:
+        _small("v_cache", v_cache, end)
 
 
-class _Same:
+class _Here:
+    """The context of a call whose tensors are on the current device."""
+
     def __enter__(self):
         pass
 
@@ -291,12 +291,24 @@ class _Same:
         pass
 
 
-_same = _Same()
+_here = _Here()
+
+
+def _on(t):
+    """(device index, the context in which a call for tensors on it launches)"""
+    index = t.get_device()
+    if index < 0:
+        raise _lib.NimllmAttnError("device tensor expected (there is no CPU path)")
+    return index, _here if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+# the handle of the current stream, without building a Stream object (3 us) where torch has a way
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _scratch(nbytes, device):
     # from the caching allocator of the current stream, so calls on two streams or in two graphs never share it
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def rope_tables_scaled(max_pos: int, rot_dim: int, base: float, *, kind="none", factor=1.0, low=1.0, high=32.0, orig_len=0,
@@ -313,24 +325,40 @@ def rope_tables_scaled(max_pos: int, rot_dim: int, base: float, *, kind="none", 
     return torch.from_numpy(cos).to(device), torch.from_numpy(sin).to(device)
 
 
-def _rope_at(q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out, k_out, want_k, has_cache):
-    if k_new is None:
-        raise _lib.NimllmAttnError("k_new is required")
-    B, n = k_new.shape[0], k_new.shape[1]
+_F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+
+
+def _rope_at(index, q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out, k_out, want_k, has_cache):
+    B, n = k_new.shape[:2]
     if q is not None and q_out is None:
         q_out = torch.empty_like(q)
     if k_out is None and (want_k or not has_cache):
         k_out = torch.empty_like(k_new)
-    act, kv = k_new.dtype, B * n * n_kv_head * head_dim
-    qs = B * n * n_head * head_dim
-    _sizes(q=(q, qs), q_out=(q_out, qs), k_new=(k_new, kv), k_out=(k_out, kv), v_new=(v_new, kv), pos=(pos, B * n), row0=(row0, B))
-    if cos is not None and sin is not None and cos.shape != sin.shape:
-        raise _lib.NimllmAttnError("cos and sin differ in shape")
-    p = _args(k_new.device, (act, act, None, act, act, torch.float32, torch.float32, torch.int32, torch.int32),
-              q, q_out, k_new, k_out, v_new, cos, sin, pos, row0)
-    rot, rows = (2 * cos.shape[1], cos.shape[0]) if cos is not None else (0, 0)
-    head = (p[0], p[1], n_head, p[2], p[3], p[4], _code(k_new), p[5], p[6], rot, _layout(layout), rows, p[7], p[8])
-    return B, n, q_out if q is not None else None, k_out, head
+    act, tokens = k_new.dtype, B * n
+    qs, kv = tokens * n_head * head_dim, tokens * n_kv_head * head_dim
+    p = _args(index, (act, act, act, act, act, _F32, _F32, _I32, _I32), (q, q_out, k_new, k_out, v_new, cos, sin, pos, row0))
+    if q is not None:
+        if q.numel() < qs:
+            _small("q", q, qs)
+        if q_out.numel() < qs:
+            _small("q_out", q_out, qs)
+    if k_new.numel() < kv:
+        _small("k_new", k_new, kv)
+    if k_out is not None and k_out.numel() < kv:
+        _small("k_out", k_out, kv)
+    if v_new is not None and v_new.numel() < kv:
+        _small("v_new", v_new, kv)
+    if pos is not None and pos.numel() < tokens:
+        _small("pos", pos, tokens)
+    if row0 is not None and row0.numel() < B:
+        _small("row0", row0, B)
+    rows = rot = 0
+    if cos is not None:
+        rows, rot = cos.shape
+        if sin is not None and sin.shape != cos.shape:
+            raise _lib.NimllmAttnError("cos and sin differ in shape")
+    return B, n, q_out if q is not None else None, k_out, (p[0], p[1], n_head, p[2], p[3], p[4], _code(k_new), p[5], p[6], 2 * rot,
+                                                           _layout(layout), rows, p[7], p[8])
 
 
 def rope_append_at(q, k_new, v_new, cos, sin, *, n_head, n_kv_head, head_dim, layout="half", pos=None, row0=None, first_row=0,
@@ -338,39 +366,49 @@ def rope_append_at(q, k_new, v_new, cos, sin, *, n_head, n_kv_head, head_dim, la
                    want_k=False):
     """Rotates q and k_new [B, n, heads*D] at pos [B, n] (int32; negative: padding, left alone) and appends k and v at the
     rows row0[b] + t.  cos/sin [rows, R/2] rotate the first R columns of every head.  Returns (q_out, k_out)."""
-    with _on(k_new.device):
-        B, n, q_out, k_out, head = _rope_at(q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out, k_out,
-                                            want_k, k_cache is not None)
+    index, here = _on(k_new)
+    with here:
+        B, n, q_out, k_out, head = _rope_at(index, q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out,
+                                            k_out, want_k, k_cache is not None)
+        kc = vc = off = None
+        code = F32
         if k_cache is not None:
-            _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
-        kc, vc, off = _args(k_new.device, (None, k_cache.dtype if k_cache is not None else None, torch.int64), k_cache, v_cache, kv_off)
-        check(lib().nimllm_rope_append_at(*head, first_row, kc, vc, _code(k_cache) if k_cache is not None else F32, off, seq_stride,
-                                          head_stride, max_seq, B, n, n_kv_head, head_dim, _stream()))
+            kc, vc, off = _args(index, (None, k_cache.dtype, _I64), (k_cache, v_cache, kv_off))
+            code = _code(k_cache)
+            if kv_off is None and v_cache is not None:
+                _check_blocks(k_cache, v_cache, _block_end(B, n_kv_head, head_dim, seq_stride, head_stride, max_seq))
+            elif kv_off is not None and kv_off.numel() < B:
+                _small("kv_off", kv_off, B)
+        check(lib().nimllm_rope_append_at(*head, first_row, kc, vc, code, off, seq_stride, head_stride, max_seq, B, n, n_kv_head, head_dim,
+                                          _raw_stream(index)))
     return q_out, k_out
 
 
-def _pages(k_pages, v_pages, page_table, batch, n_kv_head, head_dim, layers=None):
-    """(n_pages, page_rows) of pages [(layers,) n_pages, Hkv, page_rows, D], checked against the heads and the table."""
-    want = k_pages.shape[-4:]
-    if k_pages.dim() not in (4, 5) or want[1] != n_kv_head or want[3] != head_dim or v_pages.shape != k_pages.shape:
-        raise _lib.NimllmAttnError(f"pages {tuple(k_pages.shape)} / {tuple(v_pages.shape)}: [n_pages, {n_kv_head}, page_rows, {head_dim}] expected")
-    if (k_pages.shape[0] if k_pages.dim() == 5 else 1) < (layers or 1):
-        raise _lib.NimllmAttnError(f"pages {tuple(k_pages.shape)}: {layers} layers expected")
+def _pages(index, k_pages, v_pages, page_table, batch, n_kv_head, head_dim, layers=1):
+    """(pointers of K, V and the table, max_pages, page_rows, n_pages) of pages [(layers,) n_pages, Hkv, page_rows, D], checked
+    against the heads and the table."""
+    shape = k_pages.shape
+    n_pages, heads, page_rows, width = shape[-4:]
+    if len(shape) not in (4, 5) or heads != n_kv_head or width != head_dim or v_pages.shape != shape:
+        raise _lib.NimllmAttnError(f"pages {tuple(shape)} / {tuple(v_pages.shape)}: [n_pages, {n_kv_head}, page_rows, {head_dim}] expected")
+    if (shape[0] if len(shape) == 5 else 1) < layers:
+        raise _lib.NimllmAttnError(f"pages {tuple(shape)}: {layers} layers expected")
     if page_table.dim() != 2 or page_table.shape[0] < batch:
         raise _lib.NimllmAttnError(f"page_table {tuple(page_table.shape)}: [{batch}, max_pages] expected")
-    return want[0], want[2]
+    kp, vp, pt = _args(index, (None, k_pages.dtype, _I32), (k_pages, v_pages, page_table))
+    return kp, vp, pt, page_table.shape[1], page_rows, n_pages
 
 
 def rope_append_at_paged(q, k_new, v_new, cos, sin, k_pages, v_pages, page_table, *, n_head, n_kv_head, head_dim, layout="half",
                          pos=None, row0=None, first_row=0, q_out=None, k_out=None, want_k=False):
     """rope_append_at into pages [n_pages, Hkv, page_rows, D] with page_table int32 [B, max_pages]."""
-    with _on(k_new.device):
-        B, n, q_out, k_out, head = _rope_at(q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out, k_out,
-                                            want_k, True)
-        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
-        kp, vp, pt = _args(k_new.device, (None, k_pages.dtype, torch.int32), k_pages, v_pages, page_table)
-        check(lib().nimllm_rope_append_at_paged(*head, first_row, kp, vp, _code(k_pages), pt, page_table.shape[1], page_rows, n_pages,
-                                                B, n, n_kv_head, head_dim, _stream()))
+    index, here = _on(k_new)
+    with here:
+        B, n, q_out, k_out, head = _rope_at(index, q, k_new, v_new, cos, sin, n_head, n_kv_head, head_dim, layout, pos, row0, q_out,
+                                            k_out, want_k, True)
+        kp, vp, pt, max_pages, page_rows, n_pages = _pages(index, k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        check(lib().nimllm_rope_append_at_paged(*head, first_row, kp, vp, _code(k_pages), pt, max_pages, page_rows, n_pages, B, n, n_kv_head,
+                                                head_dim, _raw_stream(index)))
     return q_out, k_out
 
 
@@ -380,29 +418,45 @@ def rope_at_backward(dq_rot, dk_rot, cos, sin, *, n_head, n_kv_head, head_dim, l
     some = dq_rot if dq_rot is not None else dk_rot
     if some is None:
         raise _lib.NimllmAttnError("dq_rot or dk_rot is required")
-    B, n = some.shape[0], some.shape[1]
-    with _on(some.device):
+    B, n = some.shape[:2]
+    index, here = _on(some)
+    with here:
         dq = dq_rot if in_place or dq_rot is None else torch.empty_like(dq_rot)
         dk = dk_rot if in_place or dk_rot is None else torch.empty_like(dk_rot)
-        _sizes(dq_rot=(dq_rot, B * n * n_head * head_dim), dk_rot=(dk_rot, B * n * n_kv_head * head_dim), pos=(pos, B * n))
+        if dq_rot is not None and dq_rot.numel() < B * n * n_head * head_dim:
+            _small("dq_rot", dq_rot, B * n * n_head * head_dim)
+        if dk_rot is not None and dk_rot.numel() < B * n * n_kv_head * head_dim:
+            _small("dk_rot", dk_rot, B * n * n_kv_head * head_dim)
+        if pos is not None and pos.numel() < B * n:
+            _small("pos", pos, B * n)
         if cos.shape != sin.shape:
             raise _lib.NimllmAttnError("cos and sin differ in shape")
         dt = some.dtype
-        p = _args(some.device, (dt, dt, dt, dt, torch.float32, torch.float32, torch.int32), dq_rot, dq, dk_rot, dk, cos, sin, pos)
+        p = _args(index, (dt, dt, dt, dt, _F32, _F32, _I32), (dq_rot, dq, dk_rot, dk, cos, sin, pos))
         check(lib().nimllm_rope_at_bwd(p[0], p[1], n_head, p[2], p[3], _code(some), p[4], p[5], 2 * cos.shape[1], _layout(layout),
-                                       cos.shape[0], p[6], pos0, B, n, n_kv_head, head_dim, _stream()))
+                                       cos.shape[0], p[6], pos0, B, n, n_kv_head, head_dim, _raw_stream(index)))
     return dq, dk
 
 
-def _tree_io(q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim):
-    B, n = q.shape[0], q.shape[1]
+def _tree_io(index, q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim):
+    B, n = q.shape[:2]
+    size = B * n * n_head * head_dim
     if out is None:
         # with n_new the rows of padding tokens are not written
         out = (torch.empty if n_new is None else torch.zeros)((B, n, n_head * head_dim), dtype=out_dtype, device=q.device)
     rec = torch.empty((B * n * n_head, head_dim + 4), dtype=torch.float32, device=q.device) if partials else None
-    size = B * n * n_head * head_dim
-    _sizes(q=(q, size), out=(out, size), n_new=(n_new, B), tree_mask=(tree_mask, B * n * ((n + 63) // 64)), seq_len=(seq_len, B))
-    return B, n, out, rec
+    p = _args(index, (None, _I32, _I32, _I64, None, _F32), (q, seq_len, n_new, tree_mask, out, rec))
+    if q.numel() < size:
+        _small("q", q, size)
+    if out.numel() < size:
+        _small("out", out, size)
+    if seq_len is not None and seq_len.numel() < B:
+        _small("seq_len", seq_len, B)
+    if n_new is not None and n_new.numel() < B:
+        _small("n_new", n_new, B)
+    if tree_mask is not None and tree_mask.numel() < B * n * ((n + 63) // 64):
+        _small("tree_mask", tree_mask, B * n * ((n + 63) // 64))
+    return B, n, out, rec, p
 
 
 def decode_tree(q, k_cache, v_cache, *, n_head, n_kv_head, head_dim, max_len, max_seq, seq_len=None, n_new=None, tree_mask=None,
@@ -411,17 +465,20 @@ def decode_tree(q, k_cache, v_cache, *, n_head, n_kv_head, head_dim, max_len, ma
     draft rows seq_len[b] + j with bit j set in tree_mask [B, n, ceil(n/64)] (int64; None: drafts 0 .. i).  Returns out
     [B, n, Hq*D] (and the (o, m, l) records [B*n*Hq, D+4] when partials=True)."""
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-    with _on(q.device):
-        B, n, out, rec = _tree_io(q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim)
-        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
-        p = _args(q.device, (None, None, k_cache.dtype, torch.int64, torch.int32, torch.int32, torch.int64, None),
-                  q, k_cache, v_cache, kv_off, seq_len, n_new, tree_mask, out)
-        code = _code(k_cache)
-        need = lib().nimllm_attn_decode_tree_workspace_bytes(B, n, n_head, n_kv_head, head_dim, max_len, code)
-        ws = _scratch(need, q.device)
-        check(lib().nimllm_attn_decode_tree(
-            p[0], _code(q), p[1], p[2], code, p[3], seq_stride, head_stride, max_seq, p[4], max_len, p[5], p[6], p[7], _code(out),
-            _ptr(rec), B, n, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+    index, here = _on(q)
+    with here:
+        B, n, out, rec, p = _tree_io(index, q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim)
+        kc, vc, off = _args(index, (None, k_cache.dtype, _I64), (k_cache, v_cache, kv_off))
+        if kv_off is None:
+            _check_blocks(k_cache, v_cache, _block_end(B, n_kv_head, head_dim, seq_stride, head_stride, max_seq))
+        elif kv_off.numel() < B:
+            _small("kv_off", kv_off, B)
+        code, L = _code(k_cache), lib()
+        need = L.nimllm_attn_decode_tree_workspace_bytes(B, n, n_head, n_kv_head, head_dim, max_len, code)
+        ws = _scratch(need, q.device) if need else None
+        check(L.nimllm_attn_decode_tree(
+            p[0], _code(q), kc, vc, code, off, seq_stride, head_stride, max_seq, p[1], max_len, p[2], p[3], p[4], _code(out), p[5], B, n,
+            n_head, n_kv_head, head_dim, scale, ws.data_ptr() if need else None, need, _raw_stream(index)))
     return (out, rec) if partials else out
 
 
@@ -429,17 +486,16 @@ def decode_tree_paged(q, k_pages, v_pages, page_table, *, n_head, n_kv_head, hea
                       tree_mask=None, scale=None, out=None, out_dtype=torch.float32, partials=False):
     """decode_tree over pages [n_pages, Hkv, page_rows, D] with page_table int32 [B, max_pages]."""
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-    with _on(q.device):
-        B, n, out, rec = _tree_io(q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim)
-        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
-        p = _args(q.device, (None, None, k_pages.dtype, torch.int32, torch.int32, torch.int32, torch.int64, None),
-                  q, k_pages, v_pages, page_table, seq_len, n_new, tree_mask, out)
-        code = _code(k_pages)
-        need = lib().nimllm_attn_decode_tree_workspace_bytes(B, n, n_head, n_kv_head, head_dim, max_len, code)
-        ws = _scratch(need, q.device)
-        check(lib().nimllm_attn_decode_tree_paged(
-            p[0], _code(q), p[1], p[2], code, p[3], page_table.shape[1], page_rows, n_pages, p[4], max_len, p[5], p[6], p[7],
-            _code(out), _ptr(rec), B, n, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+    index, here = _on(q)
+    with here:
+        B, n, out, rec, p = _tree_io(index, q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_head, head_dim)
+        kp, vp, pt, max_pages, page_rows, n_pages = _pages(index, k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        code, L = _code(k_pages), lib()
+        need = L.nimllm_attn_decode_tree_workspace_bytes(B, n, n_head, n_kv_head, head_dim, max_len, code)
+        ws = _scratch(need, q.device) if need else None
+        check(L.nimllm_attn_decode_tree_paged(
+            p[0], _code(q), kp, vp, code, pt, max_pages, page_rows, n_pages, p[1], max_len, p[2], p[3], p[4], _code(out), p[5], B, n, n_head,
+            n_kv_head, head_dim, scale, ws.data_ptr() if need else None, need, _raw_stream(index)))
     return (out, rec) if partials else out
 
 
@@ -452,47 +508,59 @@ def decode_tree_status(reset: bool = True) -> int:
     return rc
 
 
-def _accept_io(path, n_path, seq_len, new_len):
+def _accept_io(index, path, n_path, seq_len, new_len):
     B, max_path = path.shape
     new_len = torch.empty_like(seq_len) if new_len is None else new_len
-    _sizes(n_path=(n_path, B), seq_len=(seq_len, B), new_len=(new_len, B))
-    i = torch.int32
-    return B, max_path, new_len, _args(path.device, (i, i, i, i), path, n_path, seq_len, new_len)
+    p = _args(index, (_I32, _I32, _I32, _I32), (path, n_path, seq_len, new_len))
+    if n_path.numel() < B or seq_len.numel() < B or new_len.numel() < B:
+        raise _lib.NimllmAttnError(f"n_path, seq_len and new_len hold {B} elements each")
+    return B, max_path, new_len, p
 
 
 def kv_accept(k_cache, v_cache, path, n_path, seq_len, *, n_draft, n_kv_head, head_dim, max_seq, n_layer=1, layer_stride=0,
               kv_off=None, seq_stride=0, head_stride=0, new_len=None):
     """Moves the rows of the accepted drafts path[b][:n_path[b]] (int32 [B, max_path], increasing) down to the rows from
     seq_len[b] on, in n_layer layers, and returns new_len [B] (given: written there; it may be seq_len)."""
-    with _on(path.device):
-        B, max_path, new_len, p = _accept_io(path, n_path, seq_len, new_len)
-        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq, n_layer, layer_stride)
-        kc, vc, off = _args(path.device, (None, k_cache.dtype, torch.int64), k_cache, v_cache, kv_off)
+    index, here = _on(path)
+    with here:
+        B, max_path, new_len, p = _accept_io(index, path, n_path, seq_len, new_len)
+        kc, vc, off = _args(index, (None, k_cache.dtype, _I64), (k_cache, v_cache, kv_off))
+        if kv_off is None:
+            _check_blocks(k_cache, v_cache, _block_end(B, n_kv_head, head_dim, seq_stride, head_stride, max_seq, n_layer, layer_stride))
+        elif kv_off.numel() < B:
+            _small("kv_off", kv_off, B)
         check(lib().nimllm_kv_accept(kc, vc, _code(k_cache), n_layer, layer_stride, off, seq_stride, head_stride, max_seq, p[0],
-                                     max_path, p[1], p[2], p[3], n_draft, B, n_kv_head, head_dim, _stream()))
+                                     max_path, p[1], p[2], p[3], n_draft, B, n_kv_head, head_dim, _raw_stream(index)))
     return new_len
 
 
 def kv_accept_paged(k_pages, v_pages, page_table, path, n_path, seq_len, *, n_draft, n_kv_head, head_dim, n_layer=1, new_len=None):
     """kv_accept over pages [(n_layer,) n_pages, Hkv, page_rows, D]; all layers share the page table."""
-    with _on(path.device):
-        B, max_path, new_len, p = _accept_io(path, n_path, seq_len, new_len)
-        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim, n_layer)
-        kp, vp, pt = _args(path.device, (None, k_pages.dtype, torch.int32), k_pages, v_pages, page_table)
-        check(lib().nimllm_kv_accept_paged(kp, vp, _code(k_pages), n_layer, n_pages * n_kv_head * page_rows * head_dim, pt,
-                                           page_table.shape[1], page_rows, n_pages, p[0], max_path, p[1], p[2], p[3], n_draft, B,
-                                           n_kv_head, head_dim, _stream()))
+    index, here = _on(path)
+    with here:
+        B, max_path, new_len, p = _accept_io(index, path, n_path, seq_len, new_len)
+        kp, vp, pt, max_pages, page_rows, n_pages = _pages(index, k_pages, v_pages, page_table, B, n_kv_head, head_dim, n_layer)
+        check(lib().nimllm_kv_accept_paged(kp, vp, _code(k_pages), n_layer, n_pages * n_kv_head * page_rows * head_dim, pt, max_pages,
+                                           page_rows, n_pages, p[0], max_path, p[1], p[2], p[3], n_draft, B, n_kv_head, head_dim,
+                                           _raw_stream(index)))
     return new_len
 
 
-def _scored_io(q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim):
-    B = q.shape[0]
-    if score.dim() != 3 or score.shape[0] < B or score.shape[1] != n_kv_head:
-        raise _lib.NimllmAttnError(f"score {tuple(score.shape)}: [{B}, {n_kv_head}, rows] expected")
+def _scored_io(index, q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim):
+    B, size = q.shape[0], q.shape[0] * n_head * head_dim
+    shape = score.shape
+    if len(shape) != 3 or shape[0] < B or shape[1] != n_kv_head:
+        raise _lib.NimllmAttnError(f"score {tuple(shape)}: [{B}, {n_kv_head}, rows] expected")
     if out is None:
         out = torch.empty((B, n_head * head_dim), dtype=out_dtype, device=q.device)
-    _sizes(q=(q, B * n_head * head_dim), out=(out, B * n_head * head_dim), seq_len=(seq_len, B))
-    return B, out
+    p = _args(index, (None, _I32, None, _F32), (q, seq_len, out, score))
+    if q.numel() < size:
+        _small("q", q, size)
+    if out.numel() < size:
+        _small("out", out, size)
+    if seq_len is not None and seq_len.numel() < B:
+        _small("seq_len", seq_len, B)
+    return B, out, shape[2], p
 
 
 def decode_scored(q, k_cache, v_cache, score, *, n_head, n_kv_head, head_dim, max_len, max_seq, seq_len=None, decay=1.0, kv_off=None,
@@ -500,17 +568,20 @@ def decode_scored(q, k_cache, v_cache, score, *, n_head, n_kv_head, head_dim, ma
     """decode_batch that also updates score [B, Hkv, rows] (fp32): decay * score + the softmax weights of the query heads
     of each KV head, summed.  Returns out [B, Hq*D]."""
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-    with _on(q.device):
-        B, out = _scored_io(q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim)
-        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
-        p = _args(q.device, (None, None, k_cache.dtype, torch.int64, torch.int32, None, torch.float32),
-                  q, k_cache, v_cache, kv_off, seq_len, out, score)
-        code = _code(k_cache)
-        need = lib().nimllm_attn_decode_scored_workspace_bytes(B, n_head, n_kv_head, head_dim, max_len, code)
+    index, here = _on(q)
+    with here:
+        B, out, score_rows, p = _scored_io(index, q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim)
+        kc, vc, off = _args(index, (None, k_cache.dtype, _I64), (k_cache, v_cache, kv_off))
+        if kv_off is None:
+            _check_blocks(k_cache, v_cache, _block_end(B, n_kv_head, head_dim, seq_stride, head_stride, max_seq))
+        elif kv_off.numel() < B:
+            _small("kv_off", kv_off, B)
+        code, L = _code(k_cache), lib()
+        need = L.nimllm_attn_decode_scored_workspace_bytes(B, n_head, n_kv_head, head_dim, max_len, code)
         ws = _scratch(need, q.device)
-        check(lib().nimllm_attn_decode_scored(
-            p[0], _code(q), p[1], p[2], code, p[3], seq_stride, head_stride, max_seq, p[4], max_len, p[5], _code(out), p[6],
-            score.shape[2], decay, B, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+        check(L.nimllm_attn_decode_scored(
+            p[0], _code(q), kc, vc, code, off, seq_stride, head_stride, max_seq, p[1], max_len, p[2], _code(out), p[3], score_rows, decay,
+            B, n_head, n_kv_head, head_dim, scale, ws.data_ptr(), need, _raw_stream(index)))
     return out
 
 
@@ -518,55 +589,62 @@ def decode_scored_paged(q, k_pages, v_pages, page_table, score, *, n_head, n_kv_
                         scale=None, out=None, out_dtype=torch.float32):
     """decode_scored over pages [n_pages, Hkv, page_rows, D] with page_table int32 [B, max_pages]."""
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-    with _on(q.device):
-        B, out = _scored_io(q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim)
-        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
-        p = _args(q.device, (None, None, k_pages.dtype, torch.int32, torch.int32, None, torch.float32),
-                  q, k_pages, v_pages, page_table, seq_len, out, score)
-        code = _code(k_pages)
-        need = lib().nimllm_attn_decode_scored_workspace_bytes(B, n_head, n_kv_head, head_dim, max_len, code)
+    index, here = _on(q)
+    with here:
+        B, out, score_rows, p = _scored_io(index, q, score, seq_len, out, out_dtype, n_head, n_kv_head, head_dim)
+        kp, vp, pt, max_pages, page_rows, n_pages = _pages(index, k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        code, L = _code(k_pages), lib()
+        need = L.nimllm_attn_decode_scored_workspace_bytes(B, n_head, n_kv_head, head_dim, max_len, code)
         ws = _scratch(need, q.device)
-        check(lib().nimllm_attn_decode_scored_paged(
-            p[0], _code(q), p[1], p[2], code, p[3], page_table.shape[1], page_rows, n_pages, p[4], max_len, p[5], _code(out), p[6],
-            score.shape[2], decay, B, n_head, n_kv_head, head_dim, scale, _ptr(ws), need, _stream()))
+        check(L.nimllm_attn_decode_scored_paged(
+            p[0], _code(q), kp, vp, code, pt, max_pages, page_rows, n_pages, p[1], max_len, p[2], _code(out), p[3], score_rows, decay, B,
+            n_head, n_kv_head, head_dim, scale, ws.data_ptr(), need, _raw_stream(index)))
     return out
 
 
-def _evict_io(score, seq_len, keep, kept, new_len, n_kv_head, batch):
-    B = score.shape[0] if batch is None else batch
-    if score.dim() != 3 or score.shape[0] < B or score.shape[1] != n_kv_head:
-        raise _lib.NimllmAttnError(f"score {tuple(score.shape)}: [{B}, {n_kv_head}, rows] expected")
+def _evict_io(index, score, seq_len, keep, kept, new_len, n_kv_head, batch):
+    shape = score.shape
+    B = shape[0] if batch is None else batch
+    if len(shape) != 3 or shape[0] < B or shape[1] != n_kv_head:
+        raise _lib.NimllmAttnError(f"score {tuple(shape)}: [{B}, {n_kv_head}, rows] expected")
     if kept is None:
-        kept = torch.empty((B, n_kv_head, max(keep, 0)), dtype=torch.int32, device=score.device)
+        kept = torch.empty((B, n_kv_head, max(keep, 0)), dtype=_I32, device=score.device)
     if new_len is None:
-        new_len = torch.empty(B, dtype=torch.int32, device=score.device)
-    _sizes(seq_len=(seq_len, B), kept=(kept, B * n_kv_head * keep), new_len=(new_len, B))
-    i = torch.int32
-    return B, kept, new_len, _args(score.device, (torch.float32, i, i, i), score, seq_len, kept, new_len)
+        new_len = torch.empty(B, dtype=_I32, device=score.device)
+    p = _args(index, (_F32, _I32, _I32, _I32), (score, seq_len, kept, new_len))
+    if kept.numel() < B * n_kv_head * keep:
+        _small("kept", kept, B * n_kv_head * keep)
+    if new_len.numel() < B or (seq_len is not None and seq_len.numel() < B):
+        raise _lib.NimllmAttnError(f"seq_len and new_len hold {B} elements each")
+    return B, shape[2], kept, new_len, p
 
 
 def kv_evict(k_cache, v_cache, score, seq_len, *, keep, n_kv_head, head_dim, max_len, max_seq, n_sink=0, n_recent=0, kv_off=None,
              seq_stride=0, head_stride=0, kept=None, new_len=None, batch=None):
     """Cuts every sequence to `keep` rows: per KV head the first n_sink, the last n_recent and those with the largest
     score [B, Hkv, rows] in between, in order; K, V and score move.  Returns (new_len [B], kept [B, Hkv, keep])."""
-    with _on(score.device):
-        B, kept, new_len, p = _evict_io(score, seq_len, keep, kept, new_len, n_kv_head, batch)
-        _block_sizes(k_cache, v_cache, kv_off, B, n_kv_head, head_dim, seq_stride, head_stride, max_seq)
-        kc, vc, off = _args(score.device, (None, k_cache.dtype, torch.int64), k_cache, v_cache, kv_off)
-        check(lib().nimllm_kv_evict(kc, vc, _code(k_cache), off, seq_stride, head_stride, max_seq, p[0], score.shape[2], p[1], max_len,
-                                    keep, n_sink, n_recent, p[2], p[3], B, n_kv_head, head_dim, _stream()))
+    index, here = _on(score)
+    with here:
+        B, score_rows, kept, new_len, p = _evict_io(index, score, seq_len, keep, kept, new_len, n_kv_head, batch)
+        kc, vc, off = _args(index, (None, k_cache.dtype, _I64), (k_cache, v_cache, kv_off))
+        if kv_off is None:
+            _check_blocks(k_cache, v_cache, _block_end(B, n_kv_head, head_dim, seq_stride, head_stride, max_seq))
+        elif kv_off.numel() < B:
+            _small("kv_off", kv_off, B)
+        check(lib().nimllm_kv_evict(kc, vc, _code(k_cache), off, seq_stride, head_stride, max_seq, p[0], score_rows, p[1], max_len,
+                                    keep, n_sink, n_recent, p[2], p[3], B, n_kv_head, head_dim, _raw_stream(index)))
     return new_len, kept
 
 
 def kv_evict_paged(k_pages, v_pages, page_table, score, seq_len, *, keep, n_kv_head, head_dim, max_len, n_sink=0, n_recent=0, kept=None,
                    new_len=None, batch=None):
     """kv_evict over pages [n_pages, Hkv, page_rows, D]; give the empty pages back with PagedKvPool.shrink."""
-    with _on(score.device):
-        B, kept, new_len, p = _evict_io(score, seq_len, keep, kept, new_len, n_kv_head, batch)
-        n_pages, page_rows = _pages(k_pages, v_pages, page_table, B, n_kv_head, head_dim)
-        kp, vp, pt = _args(score.device, (None, k_pages.dtype, torch.int32), k_pages, v_pages, page_table)
-        check(lib().nimllm_kv_evict_paged(kp, vp, _code(k_pages), pt, page_table.shape[1], page_rows, n_pages, p[0], score.shape[2], p[1],
-                                          max_len, keep, n_sink, n_recent, p[2], p[3], B, n_kv_head, head_dim, _stream()))
+    index, here = _on(score)
+    with here:
+        B, score_rows, kept, new_len, p = _evict_io(index, score, seq_len, keep, kept, new_len, n_kv_head, batch)
+        kp, vp, pt, max_pages, page_rows, n_pages = _pages(index, k_pages, v_pages, page_table, B, n_kv_head, head_dim)
+        check(lib().nimllm_kv_evict_paged(kp, vp, _code(k_pages), pt, max_pages, page_rows, n_pages, p[0], score_rows, p[1], max_len, keep,
+                                          n_sink, n_recent, p[2], p[3], B, n_kv_head, head_dim, _raw_stream(index)))
     return new_len, kept
 
 
