@@ -101,7 +101,6 @@ __device__ __forceinline__ uint64_t visible_rows(const TreeParams &p, const SegE
     return vis;
 }
 
-
 __device__ __forceinline__ uint64_t pair2(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ void unpair2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ uint64_t add2_f32(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
@@ -324,12 +323,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                     fence_async();
                     tc_fence_after();
                     const uint32_t q_lo = (((q_base + (SPLIT ? g : buf) * kQTile) >> 4) & 0x3FFFu) | kLbo;
+                    // smallest terms first: the sum is short of bits only from where the large ones have come in
 #pragma unroll
-                    for (int t = 0; t < NQ; t++)
+                    for (int t = NQ - 1; t >= 0; t--)
 #pragma unroll
                         for (int ks = 0; ks < D / 16; ks++)
                             mma_ss_if(leader, tmem + g * kGroupCols, make_desc(q_lo + t * (kQTerm >> 4) + (ks >> 2) * (kQBox >> 4) + (ks & 3) * 2, kDescHi),
-                                      make_desc(k_lo + (ks >> 2) * (kKvBox >> 4) + (ks & 3) * 2, kDescHi), idesc, (t > 0 || ks > 0) ? 1u : 0u);
+                                      make_desc(k_lo + (ks >> 2) * (kKvBox >> 4) + (ks & 3) * 2, kDescHi), idesc, (t < NQ - 1 || ks > 0) ? 1u : 0u);
                     tc_commit_if(leader, &sb.s_full[g]);
                 }
                 if (!ok) break;
@@ -362,12 +362,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                     tc_fence_after();
                     const uint32_t at = tmem + g * kGroupCols;
 #pragma unroll
-                    for (int t = 0; t < NP; t++)
+                    for (int t = NP - 1; t >= 0; t--)
 #pragma unroll
                         for (int ks = 0; ks < kTile / 16; ks++) {
                             // P: 8 packed columns a step (fp32 results: two terms over the 32 columns of S that they came from)
                             const uint32_t pa = NP == 3 && t < 2 ? at + (ks >> 1) * 32 + t * 16 + (ks & 1) * 8 : at + kColP + (NP == 3 ? 0 : t * 32) + ks * 8;
-                            mma_ts_if(leader, at + kColO, pa, make_desc(v_lo + ks * 128, kDescHi), idesc, t > 0 || ks > 0 || jg % kOWindow != 0 ? 1u : 0u);
+                            mma_ts_if(leader, at + kColO, pa, make_desc(v_lo + ks * 128, kDescHi), idesc, t < NP - 1 || ks > 0 || jg % kOWindow != 0 ? 1u : 0u);
                         }
                     tc_commit_if(leader, &sb.pv_done[g]);
                 }
