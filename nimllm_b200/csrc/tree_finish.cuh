@@ -14,21 +14,24 @@ constexpr int kMaxPieces = 180;        // 32 rows of them in 48 KB
 
 // The pieces of a query row.  Tensor-core kernels: records of consecutive CTAs (tree_tc.cuh); CUDA-core kernel: one record per chunk of
 // rows.  n = 1: the kernel stored the row itself; n = 0: there was nothing to attend.
+// Column d of row r is at rec(i) + r * row + d / 4 * col + d % 4, its maximum and sum where column D would be.
 struct Pieces {
     int n;
     const float *first, *second;       // record of piece 0, of piece 1; the others follow at `step`
     int64_t step;
+    int row, col;
     __device__ const float *rec(int x) const { return x == 0 ? first : second + (x - 1) * step; }
 };
 struct FinishArgs {
     TcArgs tc;
     int rpt, tile, workers;            // tensor-core kernels; workers = 0: the chunks of the CUDA-core kernel
+    bool by_col;                       // the records are [D / 4 + 1][row][4], as a thread per row stores them best
     int n_join, n_zero;                // blocks of the first two kinds
 };
 
 template <int D> __device__ __forceinline__ Pieces tc_pieces(const TreeParams &p, const FinishArgs &f, int b, int kvh, int qr, int total, int R) {
     constexpr int W = D + 4;
-    Pieces x{0, nullptr, nullptr, 0};
+    Pieces x{0, nullptr, nullptr, 0, f.by_col ? 4 : W, f.by_col ? 4 * f.tc.rec_rows : 4};
     if (total == 0) return x;
     const int64_t T = f.tc.cum[p.B];
     const int wa = (int)(T < f.workers ? T : f.workers);
@@ -38,13 +41,14 @@ template <int D> __device__ __forceinline__ Pieces tc_pieces(const TreeParams &p
     const int w0 = owner_of(s, T, wa);
     x.n = owner_of(s + tiles - 1, T, wa) - w0 + 1;
     x.step = (int64_t)2 * f.tc.rec_rows * W;
-    x.first = p.recs + ((int64_t)w0 * 2 + (first_unit(w0, T, wa) < s ? 1 : 0)) * f.tc.rec_rows * W + r * W;
-    x.second = p.recs + ((int64_t)(w0 + 1) * 2) * f.tc.rec_rows * W + r * W;
+    x.first = p.recs + ((int64_t)w0 * 2 + (first_unit(w0, T, wa) < s ? 1 : 0)) * f.tc.rec_rows * W + r * x.row;
+    x.second = p.recs + ((int64_t)(w0 + 1) * 2) * f.tc.rec_rows * W + r * x.row;
     return x;
 }
 template <int D> __device__ __forceinline__ Pieces chunk_pieces(const TreeParams &p, int64_t orow, int total) {
     constexpr int W = D + 4;
     Pieces x;
+    x.row = W; x.col = 4;
     x.n = total <= p.chunk_rows ? 1 : (total + p.chunk_rows - 1) / p.chunk_rows;      // an empty row is stored by chunk 0
     x.step = (int64_t)p.B * p.n * p.Hq * W;
     x.first = p.recs + orow * W;
@@ -56,7 +60,7 @@ template <int D> __device__ __forceinline__ Pieces chunk_pieces(const TreeParams
 template <int D> __device__ __forceinline__ void pieces_stats(const Pieces &x, int lane, float &M, float &L) {
     M = -INFINITY;
     for (int i = lane; i < x.n; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2 *>(x.rec(i) + D);
+        const float2 ml = *reinterpret_cast<const float2 *>(x.rec(i) + D / 4 * x.col);
         if (ml.y > 0.f) M = fmaxf(M, ml.x);
     }
 #pragma unroll
@@ -64,14 +68,14 @@ template <int D> __device__ __forceinline__ void pieces_stats(const Pieces &x, i
     const float safe = M == -INFINITY ? 0.f : M;
     L = 0.f;
     for (int i = lane; i < x.n; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2 *>(x.rec(i) + D);
+        const float2 ml = *reinterpret_cast<const float2 *>(x.rec(i) + D / 4 * x.col);
         if (ml.y > 0.f) L += ml.y * ex2((ml.x - safe) * kLog2e);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
 }
 
-// One block joins up to 32 rows that are cut alike: piece i of row r is the record at rec(i) + r * W.  `out_row(r)` is its row of out.
+// One block joins up to 32 rows that are cut alike.  `out_row(r)` is row r's row of out.
 // First every (row, piece) statistic is fetched at once and turned into the piece's weight, then every 16 bytes of the rows is a sum
 // over the pieces whose loads wait for nothing else.
 constexpr int kJoinRows = 32;
@@ -80,7 +84,7 @@ __device__ __forceinline__ void join_rows(const TreeParams &p, const Pieces &x, 
     constexpr int W = D + 4, kLanes = kFinishThreads / kJoinRows;
     for (int e = threadIdx.x; e < rows * x.n; e += kFinishThreads) {
         const int i = e / rows, r = e - i * rows;
-        s_ml[r * x.n + i] = *reinterpret_cast<const float2 *>(x.rec(i) + r * W + D);
+        s_ml[r * x.n + i] = *reinterpret_cast<const float2 *>(x.rec(i) + r * x.row + D / 4 * x.col);
     }
     __syncthreads();
     const int r = threadIdx.x / kLanes, sub = threadIdx.x % kLanes;
@@ -105,13 +109,15 @@ __device__ __forceinline__ void join_rows(const TreeParams &p, const Pieces &x, 
         if (sub == 0 && p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + out_row(r) * W + D) = make_float4(M, L, 0.f, 0.f);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < rows * (D / 4); e += kFinishThreads) {
-        const int rr = e / (D / 4), d = e % (D / 4) * 4;
+    // a warp has four rows by eight 16-byte columns: whole sectors of records in either layout, and of out
+    for (int e = threadIdx.x; e < (rows + 3) / 4 * D; e += kFinishThreads) {
+        const int rr = e / D * 4 + (e & 3), d = e % D / 4 * 4;
+        if (rr >= rows) continue;
         const float2 *w = s_ml + rr * x.n;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int i = 0; i < x.n; i++) {
-            const float4 o = *reinterpret_cast<const float4 *>(x.rec(i) + rr * W + d);
+            const float4 o = *reinterpret_cast<const float4 *>(x.rec(i) + rr * x.row + d / 4 * x.col);
             const float f = w[i].x;
             acc.x = fmaf(f, o.x, acc.x); acc.y = fmaf(f, o.y, acc.y); acc.z = fmaf(f, o.z, acc.z); acc.w = fmaf(f, o.w, acc.w);
         }

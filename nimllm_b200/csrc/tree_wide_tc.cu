@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                 f1 *= inv;
                 m = m == kUnset ? -INFINITY : m;
                 const int64_t orow = tree_out_row(p, sg.b, sg.kvh, qr);
-                float *rec = sg.flags & 1 ? nullptr : p.recs + (((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * a.rec_rows + (SPLIT ? g * kRows : 0) + row) * W;
+                float *rec = sg.flags & 1 ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * a.rec_rows * W + ((SPLIT ? g * kRows : 0) + row) * 4;
                 const bool any1 = __any_sync(0xffffffffu, f1 != 0.f);
 #pragma unroll
                 for (int y0 = 0; y0 < D; y0 += 16) {
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                     if (live) {
                         if (rec) {
 #pragma unroll
-                            for (int y = 0; y < 16; y += 4) *reinterpret_cast<float4 *>(rec + y0 + y) = make_float4(v[y], v[y + 1], v[y + 2], v[y + 3]);
+                            for (int y = 0; y < 16; y += 4) *reinterpret_cast<float4 *>(rec + (y0 + y) * a.rec_rows) = make_float4(v[y], v[y + 1], v[y + 2], v[y + 3]);
                         } else {
 #pragma unroll
                             for (int y = 0; y < 16; y += 8) store_row8<D>(p, orow, y0 + y, v + y);
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                 }
                 if (live) {
                     if (rec) {
-                        *reinterpret_cast<float4 *>(rec + D) = make_float4(m * kLn2, l, 0.f, 0.f);
+                        *reinterpret_cast<float4 *>(rec + D * a.rec_rows) = make_float4(m * kLn2, l, 0.f, 0.f);
                         mark_cut(p, orow);
                     } else {
                         store_row_stats<D>(p, orow, m, l);
@@ -656,7 +656,7 @@ cudaError_t launch_d(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     else e = a.p_terms == 2 ? launch_wide<D, 3, 1>(p, a, st) : launch_wide<D, 3, 3>(p, a, st);
     if (e != cudaSuccess) return e;
     FinishArgs f = {};
-    f.tc = a; f.rpt = rows_per_tile(R, a.q_terms, a.p_terms, D); f.tile = narrow ? kNarrowTile : kTile; f.workers = sm_count();
+    f.tc = a; f.rpt = rows_per_tile(R, a.q_terms, a.p_terms, D); f.tile = narrow ? kNarrowTile : kTile; f.workers = sm_count(); f.by_col = !narrow;
     return launch_finish<D>(p, f, st);
 }
 
