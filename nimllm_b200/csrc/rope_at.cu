@@ -8,6 +8,9 @@
 //
 // HBM-bound elementwise work.  A thread moves pairs of vectors of V elements (16 bytes each where the head allows: V = 8 for
 // bf16, 4 for fp32; else 4), all of them rotated or all of them passed.
+//
+// Measured (graph replay): gradient of 4 x 8192 tokens, 32 + 8 heads of 128, bf16: 127 us = 5.3 TB/s; 61 trees of 24 tokens into pages:
+// 10.3 us (5.6 us of memory time, the rest is launch and two dependent loads, pos and then tables); one token 4.1 us.
 #include <math.h>
 
 #include "cache_rows.cuh"
@@ -168,7 +171,8 @@ cudaError_t launch_heads(RopeAtParams p, int layout, cudaStream_t st) {
 }
 template <typename ActT, typename CacheT, int V>
 cudaError_t launch_v(const RopeAtParams &p, int layout, cudaStream_t st) {
-    // four heads a thread once that still leaves every SM full of threads
+    // four heads a thread share the table's loads once that still leaves every SM full of threads: the gradient of 4 x 8192 tokens
+    // takes 126.9 us, 129.4 with one head a thread; a decode step of 200 tokens 4.4 us with one, 6.4 with four
     const int64_t threads = (int64_t)p.B * p.n * (p.n_q + p.n_k + p.n_v) * (p.D / (2 * V));
     return threads >= (int64_t)sm_count() * 2048 * 4 ? launch_heads<ActT, CacheT, V, 4>(p, layout, st) : launch_heads<ActT, CacheT, V, 1>(p, layout, st);
 }

@@ -7,6 +7,10 @@
 //
 // More query rows (tree_f32_tiled_kernel) are bound by the multiply-adds: a CTA has 32 or 64 query rows and one chunk of cached
 // rows, a thread a (2 or 4) x (BN / 8) block of the score tile and the same rows' D / 8 output columns, as in prefill_f32.cu.
+//
+// Measured (graph replay): scored decode of 16 sequences of 4 - 8 K rows, 32 q / 8 kv heads of 128: 144 us, 124 at the measured peak of
+// HBM; 7 drafts of one sequence of 505 rows 15 us, its next token 11 us (latency: two launches, a tile, the join); 4 trees of 64 tokens
+// over 4 - 8 K rows 774 us, 34 TFLOP/s of multiply-adds, about half of what the CUDA cores have.
 #include "tree_finish.cuh"
 
 namespace nimllm {
@@ -418,7 +422,9 @@ cudaError_t launch_tiled(TreeParams &p, int max_total, cudaStream_t st) {
     return e == cudaSuccess ? launch_finish<D>(p, f, st) : e;
 }
 
+// 8 sequences of 2 - 4 K rows, heads of 128, streamed and tiled: 4 rows 46 and 173 us, 8 rows 56 and 173, 16 rows 88 and 174
 bool narrow_rows(int R) { return R <= kNarrowRpt; }
+// the same with tiles of 32 and of 64 query rows: 32 rows 177 and 219 us, 48 rows 327 and 224, 64 rows 328 and 232
 int tile_rows(int R) { return R <= 32 ? 32 : 64; }
 
 // rows of a chunk: enough CTAs for four on every SM, whole tiles, and no more pieces of a row than a block joins

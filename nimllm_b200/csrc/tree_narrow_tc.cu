@@ -4,7 +4,12 @@
 //     S^T = K Q^T     (128 cached rows x N, one thread per cached row)
 //     O^T += V^T P^T  (head_dim x N, A = V as it lies in the cache, B = P^T written to shared memory by the softmax)
 // and N is the query rows, 16 or 32, times the bf16 terms of an fp32 q (S) or of P (O): the terms are further columns of the
-// same MMA, so that 32-bit precision costs little tensor time.  (tree_wide_tc.cu has the terms' sizes.)
+// same MMA, so that 32-bit precision costs little tensor time.  An fp32 q and the P of fp32 results have three terms (2^-26 left), the P
+// of bf16 results two (2^-17 left).
+//
+// HBM-bound.  Measured (graph replay): 256 sequences of 512 - 4096 rows, 5 tokens, 9 q / 3 kv heads of 64, fp32 q and results: 118 us,
+// of which the rows' bytes are 70 (3.9 TB/s: segments of a few tiles each, every one with its own Q, first maximum and join); scored
+// decode of 32 sequences of 2 - 8 K rows in pages, 32 q / 8 kv heads of 128, bf16: 138 us, 104 at the measured peak (4.9 TB/s).
 //
 //   warps 0-3, 4-7   two softmax groups, taking the tiles of 128 rows in turn: the waits of one hide behind the other
 //   warps 8-11       K rows (8, 9) and V rows (10, 11) into a ring of slots with cp.async, swizzled, exact to the row
@@ -618,7 +623,9 @@ template <int D> cudaError_t launch_narrow_d(const TreeParams &p, TcArgs &a, cud
 
 }  // namespace
 
-// P's terms are columns of one 64-column operand; 96 columns of Q at head size 128 would leave two slots
+// P's terms are columns of one 64-column operand; 96 columns of Q at head size 128 would leave two slots.
+// 32 sequences of 2 - 4 K rows, 32 q / 8 kv heads of 128, here and in tree_wide_tc.cu: bf16, 8 rows 76 and 106 us, 16 rows 79 and 107,
+// 24 rows 91 and 108, 32 rows 96 and 112; fp32 q and results, 8 rows 77 and 209, 16 rows 84 and 209.
 bool tree_narrow_takes(int R, int q_terms, int p_terms, int head_dim) {
     return R <= 16 || (R <= 32 && p_terms == 2 && (q_terms == 1 || head_dim == 64));
 }

@@ -20,7 +20,13 @@
 // results both are split into three bf16 terms (2^-26 left), further MMAs into the same accumulator, and O is taken from TMEM into
 // registers every few tiles: thousands of rows added up by the tensor core would lose what 32-bit results promise.  For bf16 results
 // P is rounded to bf16 like the result itself (the sum is taken of the rounded values, so that a single large weight stays exact);
-// a second term would make this kernel, which the tensor pipe bounds, a third slower (64-token trees over 16 K rows: 187 us).
+// a second term would make this kernel a third slower, whose tensor pipe has 24 products for every 256 query rows x 64 cached ones.
+//
+// Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 160 us; the rows' bytes at
+// the measured peak of HBM are 65 us, the products at the library's matrix rate 64.  A tile takes 2700 cycles: its 24 products 2200 - the
+// tensor core takes about 93 cycles for one, 64 columns wide or 128 - and its exponentials 1024 of the two groups' turns.  Tiles of
+// 128 rows, which need 16 products for the same work, were built with one S of both groups and with P over S: 179 and 199 us, because a
+// group then waits for the other's reading of S or for its own P.
 //
 // Every wait is bounded as in prefill_tc.cu: after about 2 s without progress the CTA aborts and raises the status word.
 #include "tree_finish.cuh"
