@@ -272,13 +272,14 @@ int nimllm_rope_at_bwd(const void *dq_rot, void *dq, int n_head, const void *dk_
  * of its tokens attend; its draft j is row seq_len[b] + j, already appended.
  *   q          [batch, n, n_head*head_dim] q_dtype, rotated;  out the same shape, out_dtype
  *   seq_len    device int32 [batch] in 0 .. max_len, or NULL: max_len for all
- *   n_new      device int32 [batch], drafts of each sequence, or NULL: n.  Rows of out past them are left as they were
+ *   n_new      device int32 [batch], drafts of each sequence, or NULL: n.  Rows of the outputs past them are left as they were
  *   tree_mask  device uint64 [batch, n, (n + 63) / 64]: bit j of token i's words, it attends draft j (its
  *              ancestors and itself); NULL: a chain, drafts 0 .. i.  A token without any row to attend gets zeros
  *   partials_out  optional fp32 [batch*n*n_head, head_dim + 4] records as in nimllm_attn_decode (out may be NULL then)
  *   head_dim   64 or 128.  The arithmetic is that of 32 bits for either cache type, but for bf16 results of more than 32
  *              query rows (n * n_head / n_kv_head), whose softmax weights are rounded to bf16.  Every row of V up to the
- *              last draft must be finite even where a mask hides it (a hidden row of K may hold anything)
+ *              last draft must be finite even where a mask hides it (a hidden row of K may hold anything); a row whose
+ *              scaled score is below -1e30 counts as hidden
  *   workspace  256-byte aligned, nimllm_attn_decode_tree_workspace_bytes(...) bytes
  * The kernel for bf16 caches (also that of nimllm_attn_decode_scored) bounds its internal waits, about 2 s without
  * progress; nimllm_attn_decode_tree_status tells as nimllm_attn_prefill_status does whether one gave up. */

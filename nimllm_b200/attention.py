@@ -10,6 +10,9 @@
   (no counterpart: batch 1 only)                  decode_batch(), combine()
   chat loop's reset-when-full cache policy        PagedKvPool (pages shared by many sequences),
     (src/chat.nim:86-91)                            rope_append_paged(), decode_paged()
+  (no counterpart: row == position there)         rope_append_at(), decode_tree(), kv_accept(),
+                                                    decode_scored(), kv_evict(), their _paged forms,
+                                                    rope_tables_scaled(), rope_at_backward()
 
 torch is used for device memory and streams only; every computation goes through
 libnimllm_attn.so and raises if that library is missing or reports an error."""
@@ -444,7 +447,7 @@ def _tree_io(index, q, n_new, tree_mask, seq_len, out, out_dtype, partials, n_he
     if out is None:
         # with n_new the rows of padding tokens are not written
         out = (torch.empty if n_new is None else torch.zeros)((B, n, n_head * head_dim), dtype=out_dtype, device=q.device)
-    rec = torch.empty((B * n * n_head, head_dim + 4), dtype=torch.float32, device=q.device) if partials else None
+    rec = (torch.empty if n_new is None else torch.zeros)((B * n * n_head, head_dim + 4), dtype=torch.float32, device=q.device) if partials else None
     p = _args(index, (None, _I32, _I32, _I64, None, _F32), (q, seq_len, n_new, tree_mask, out, rec))
     if q.numel() < size:
         _small("q", q, size)

@@ -639,16 +639,18 @@ cudaError_t launch_terms(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     return launch_dependent(tree_wide_kernel<D, NQ, NP, SPLIT>, dim3(sm_count()), kThreads, q + a.stages * slot + 1024, st, p, a);
 }
 
-// 256 rows share a tile where the shared memory holds their Q: not three terms of it at head size 128
-bool splits(int R, int q_terms, int head_dim) { return R > kRows && (q_terms == 1 || head_dim == 64); }
+// 256 rows share a tile where Q has one term; three leave too few slots, and at head size 64 no second Q to fetch ahead.  Measured with
+// and without: heads of 128, one term, 256 rows over 9 - 16 K 160 and 165 us, 160 rows over 2 - 4 K 105 and 110; heads of 64, three
+// terms, 192 rows 103 and 91 us
+bool splits(int R, int q_terms) { return R > kRows && q_terms == 1; }
 int rows_per_tile(int R, int q_terms, int p_terms, int head_dim) {
-    return tree_narrow_takes(R, q_terms, p_terms, head_dim) ? kNarrowRows : (splits(R, q_terms, head_dim) ? 2 * kRows : kRows);
+    return tree_narrow_takes(R, q_terms, p_terms, head_dim) ? kNarrowRows : (splits(R, q_terms) ? 2 * kRows : kRows);
 }
 
 template <int D, int NQ, int NP>
 cudaError_t launch_wide(const TreeParams &p, TcArgs &a, cudaStream_t st) {
-    if constexpr (NQ == 1 || D == 64)
-        if (splits(p.n * p.G, NQ, D)) return launch_terms<D, NQ, NP, true>(p, a, st);
+    if constexpr (NQ == 1)
+        if (splits(p.n * p.G, NQ)) return launch_terms<D, NQ, NP, true>(p, a, st);
     return launch_terms<D, NQ, NP, false>(p, a, st);
 }
 

@@ -244,3 +244,35 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for t, w in zip((a, b), want):
         assert all(torch.equal(x, y) for x, y in zip(t.state(), w))
+
+
+@pytest.mark.parametrize("dtype", [F, H])
+def test_offsets_past_32_bits(dtype):
+    """The second sequence lies 2^31 elements behind the first; the results are those of a small cache with the same rows."""
+    L, n, cap, hkv, hq, far = 200, 5, 256, 2, 4, 2 ** 31 + 64
+    big = [torch.empty(far + hkv * cap * D, dtype=dtype, device="cuda") for _ in range(2)]
+    small = [torch.empty(2, hkv, cap, D, dtype=dtype, device="cuda") for _ in range(2)]
+    off = torch.tensor([0, far], dtype=torch.int64, device="cuda")
+    there = [(0, hkv * cap * D), (far, far + hkv * cap * D)]
+    for x, y in zip(big, small):
+        y.normal_()
+        for b, (i, j) in enumerate(there):
+            x[i:j] = y[b].flatten()
+    len0 = torch.full((2,), L, dtype=torch.int32, device="cuda")
+    cos, sin = A.rope_tables_scaled(TABLE + 100, D, 10000.0)
+    q, k, v = (torch.randn(2, n, h * D, device="cuda") for h in (hq, hkv, hkv))
+    results = []
+    for (kc, vc), where in ((big, dict(kv_off=off)), (small, dict(seq_stride=hkv * cap * D))):
+        where = dict(head_stride=cap * D, max_seq=cap, **where)
+        heads = dict(n_kv_head=hkv, head_dim=D)
+        lens, score = len0.clone(), torch.rand(2, hkv, cap, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+        qr = A.rope_append_at(q, k, v, cos, sin, n_head=hq, row0=lens, k_cache=kc, v_cache=vc, **heads, **where)[0]
+        o = A.decode_tree(qr, kc, vc, n_head=hq, max_len=L, seq_len=lens, **heads, **where)
+        A.kv_accept(kc, vc, torch.tensor([[1, 3], [2, 4]], dtype=torch.int32, device="cuda"), torch.full((2,), 2, dtype=torch.int32, device="cuda"),
+                    lens, n_draft=n, new_len=lens, **heads, **where)
+        s = A.decode_scored(qr[:, 0].contiguous(), kc, vc, score, n_head=hq, max_len=L + n, seq_len=lens, **heads, **where)
+        _, kept = A.kv_evict(kc, vc, score, lens, keep=90, max_len=L + n, n_sink=4, n_recent=9, new_len=lens, **heads, **where)
+        rows = [kc[i:j].view(hkv, cap, D)[:, :90].clone() if kc.dim() == 1 else kc[b, :, :90].clone() for b, (i, j) in enumerate(there)]
+        results.append([o, s, score, kept, lens] + rows)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)

@@ -89,6 +89,13 @@ def test_tree_sizes(cache_dtype, n):
     _tree_case(14, [300, 1], n, 3, 3, 64, H, cache_dtype, H, 0, "tree", ragged=False)
 
 
+@pytest.mark.parametrize("n,G", [(48, 3), (33, 8), (7, 6)])
+@pytest.mark.parametrize("D,types", [(64, (F, H, F)), (64, (F, H, H)), (64, (H, H, H)), (128, (F, H, F)), (128, (F, H, H)), (128, (H, H, F)), (128, (H, H, H)), (64, (F, F, F))])
+def test_many_segments(D, types, n, G):
+    """More pieces than SMs, so that a CTA has several sequences, some of one token or without rows, between its cuts."""
+    _tree_case(31, [130, 0, 300, 1, 64, 257, 0, 128, 5, 190, 31, 222], n, 8 * G, 8, D, *types, 0, "tree")
+
+
 @pytest.mark.parametrize("mask", ["chain", "empty"])
 @pytest.mark.parametrize("cache_dtype", [F, H])
 def test_chain_and_tokens_without_drafts(cache_dtype, mask):
