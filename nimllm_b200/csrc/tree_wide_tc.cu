@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
         constexpr int kChunks = D / 8, kStep = 64 / kChunks;
         const int which = (warp - 8) >> 1, t = (int)threadIdx.x - 256 - which * 64, c = t % kChunks, r_in = t / kChunks;
         const uint32_t kv = smem_u32(s_kv);
+        const uint64_t policy = evict_first_policy();
         const __nv_bfloat16 *src = reinterpret_cast<const __nv_bfloat16 *>(which ? p.v : p.k) + c * 8;
         int k = 0, slot = which, phase = 1;
         for (int seg = 0; next_segment(sb, seg, sg, ok, lane); seg++) {
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                     for (int r0 = 0; r0 < 32; r0 += kStep) {
                         const int rr = y * 32 + r0 + r_in;
                         const bool have = r0 + r_in < r_end;
-                        cp_async16(dst + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), have ? g + r0 * D : src, have ? 16 : 0);
+                        cp_async16(dst + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), have ? g + r0 * D : src, have ? 16 : 0, policy);
                     }
                 }
                 cp_async_arrive(&sb.full[slot]);
