@@ -624,8 +624,9 @@ template <int D> cudaError_t launch_narrow_d(const TreeParams &p, TcArgs &a, cud
 }  // namespace
 
 // P's terms are columns of one 64-column operand; 96 columns of Q at head size 128 would leave two slots.
-// 32 sequences of 2 - 4 K rows, 32 q / 8 kv heads of 128, here and in tree_wide_tc.cu: bf16, 8 rows 76 and 106 us, 16 rows 79 and 107,
-// 24 rows 91 and 108, 32 rows 96 and 112; fp32 q and results, 8 rows 77 and 209, 16 rows 84 and 209.
+// 32 sequences of 2 - 4 K rows, 32 q / 8 kv heads of 128, here and in tree_wide_tc.cu: bf16, 8 rows 76 and 96 us, 16 rows 79 and 95,
+// 24 rows 91 and 97, 32 rows 96 and 99; fp32 q and results, 8 rows 76 and 193, 16 rows 84 and 192.  64 sequences, 9 q / 3 kv heads of 64,
+// fp32 q and bf16 results: 15 rows 47 and 72, 30 rows 69 and 74.
 bool tree_narrow_takes(int R, int q_terms, int p_terms, int head_dim) {
     return R <= 16 || (R <= 32 && p_terms == 2 && (q_terms == 1 || head_dim == 64));
 }

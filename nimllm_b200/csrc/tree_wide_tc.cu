@@ -22,11 +22,12 @@
 // P is rounded to bf16 like the result itself (the sum is taken of the rounded values, so that a single large weight stays exact);
 // a second term would make this kernel a third slower, whose tensor pipe has 24 products for every 256 query rows x 64 cached ones.
 //
-// Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 160 us; the rows' bytes at
-// the measured peak of HBM are 65 us, the products at the library's matrix rate 64.  A tile takes 2700 cycles: its 24 products 2200 - the
-// tensor core takes about 93 cycles for one, 64 columns wide or 128 - and its exponentials 1024 of the two groups' turns.  Tiles of
-// 128 rows, which need 16 products for the same work, were built with one S of both groups and with P over S: 179 and 199 us, because a
-// group then waits for the other's reading of S or for its own P.
+// Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 152 us (160 without the
+// rows' policy of leaving L2 first, which keeps records, Q and code there).  The rows' bytes at the measured peak of HBM are 65 us, the
+// products at the library's matrix rate 64.  A tile takes 2700 cycles: its 24 products 2200 - the tensor core takes about 93 cycles for
+// one, 64 columns wide or 128 - and its exponentials 1024 of the two groups' turns.  Tiles of 128 rows, which need 16 products for the
+// same work, were built with one S of both groups and with P over S, before that policy: 179 and 199 us for 168, because a group then
+// waits for the other's reading of S or for its own P.
 //
 // Every wait is bounded as in prefill_tc.cu: after about 2 s without progress the CTA aborts and raises the status word.
 #include "tree_finish.cuh"
@@ -641,8 +642,8 @@ cudaError_t launch_terms(const TreeParams &p, TcArgs &a, cudaStream_t st) {
 }
 
 // 256 rows share a tile where Q has one term; three leave too few slots, and at head size 64 no second Q to fetch ahead.  Measured with
-// and without: heads of 128, one term, 256 rows over 9 - 16 K 160 and 165 us, 160 rows over 2 - 4 K 105 and 110; heads of 64, three
-// terms, 192 rows 103 and 91 us
+// and without: heads of 128, one term, 256 rows over 9 - 16 K 152.2 and 153.4 us, 160 rows over 2 - 4 K 94.9 and 96.8; heads of 64,
+// three terms, 192 rows 103 and 91 us
 bool splits(int R, int q_terms) { return R > kRows && q_terms == 1; }
 int rows_per_tile(int R, int q_terms, int p_terms, int head_dim) {
     return tree_narrow_takes(R, q_terms, p_terms, head_dim) ? kNarrowRows : (splits(R, q_terms) ? 2 * kRows : kRows);
