@@ -224,8 +224,8 @@ void *nimllm_kvpool_v(const nimllm_kvpool *pool, int layer);
  * Every one takes the contiguous layout (kv_off / seq_stride / head_stride / max_seq rows per block)
  * or, with _paged, pages (page_rows a power of two >= 32; n_pages the size of the pool).  Rows at or
  * past max_seq (max_pages * page_rows) and rows whose table entry is outside [0, n_pages) do not
- * exist: they are not read, stored, attended or moved.  Cache pointers and strides are multiples of
- * 16 bytes.  Lengths in device arrays are clamped to what the host arguments allow.  All calls can be
+ * exist: they are not read, stored, attended or moved.  Cache pointers, strides and the offsets in kv_off
+ * are multiples of 16 bytes.  Lengths in device arrays are clamped to what the host arguments allow.  All calls can be
  * captured in a CUDA graph; calls that may overlap on the GPU need workspaces of their own. */
 #define NIMLLM_ROPE_HALF 0        /* pairs (f, f + rot_dim/2), as the reference rotates */
 #define NIMLLM_ROPE_INTERLEAVED 1 /* pairs (2f, 2f + 1) */
