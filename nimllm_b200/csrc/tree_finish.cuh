@@ -211,17 +211,18 @@ __global__ void __launch_bounds__(kFinishThreads, 4) tree_finish_kernel(TreePara
     const int len = tree_committed(p, b);
     if (r0 >= len) return;
     __syncthreads();
-    // a negative sum marks a row that was cut: its pieces are joined here (all heads of a pair are cut alike)
-    if (s_stat[0].y < 0.f) {
-        __syncthreads();
-        for (int g = warp; g < p.G; g += kFinishThreads / 32) {
-            const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g, len, p.G) : chunk_pieces<D>(p, h0 + g, len);
-            float M, L;
-            pieces_stats<D>(pc, lane, M, L);
-            if (lane == 0) s_stat[g] = make_float2(M * kLog2e, L > 0.f ? 1.f / L : 0.f);
-        }
-        __syncthreads();
+    // a negative sum marks a row that was cut: its pieces are joined here.  Every head is asked by itself: heads in different query tiles
+    // (128 or 256 of them) are cut apart from one another.  A head's entry is read and written by one warp.
+    for (int g = warp; g < p.G; g += kFinishThreads / 32) {
+        const bool cut = s_stat[g].y < 0.f;
+        __syncwarp();
+        if (!cut) continue;
+        const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g, len, p.G) : chunk_pieces<D>(p, h0 + g, len);
+        float M, L;
+        pieces_stats<D>(pc, lane, M, L);
+        if (lane == 0) s_stat[g] = make_float2(M * kLog2e, L > 0.f ? 1.f / L : 0.f);
     }
+    __syncthreads();
     for (; row < min(len, r0 + kScoreRows); row += 4 * kFinishThreads) {
         Ahead next;
         if (row + 4 * kFinishThreads < min(len, r0 + kScoreRows)) fetch(next, row + 4 * kFinishThreads);
