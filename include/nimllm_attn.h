@@ -300,7 +300,8 @@ int nimllm_attn_decode_tree_paged(const void *q, int q_dtype, const void *k_page
 /* After the drafts were checked: row seq_len[b] + i of K and V becomes the former row seq_len[b] + path[b][i], for
  * i < n_path[b], in n_layer layers that lie layer_stride elements apart, and new_len[b] = seq_len[b] + the number of
  * accepted rows (new_len may be seq_len).  A path lists its drafts from the root down, so its entries increase; it ends
- * early at an entry that does not, or that is not in 0 .. n-1.
+ * early at an entry that does not, or that is not in 0 .. n-1.  Rows move in place, so the blocks of two layers, sequences or KV
+ * heads must not overlap (strides with which they do are refused), nor may sequences of the call share a page; nimllm_kv_evict too.
  *   path  device int32 [batch, max_path], max_path <= n <= 256;  n_path, seq_len, new_len  device int32 [batch] */
 int nimllm_kv_accept(void *k_cache, void *v_cache, int cache_dtype, int n_layer, int64_t layer_stride,
                      const int64_t *kv_off, int64_t seq_stride, int64_t head_stride, int max_seq, const int32_t *path,

@@ -58,6 +58,41 @@ inline int paged_rows(CacheRows &c, const char *who, const void *k, const void *
     return NIMLLM_OK;
 }
 
+// True when no two blocks of `block` elements overlap that lie stride[i] apart in each of three directions, count[i] of them (moves in
+// place by a thread block per cache block race with one another otherwise).  Strides that nest, each one clear of all that the
+// smaller ones reach over, are apart; for others every difference of two blocks is looked at.
+inline bool blocks_apart(int64_t block, const int64_t (&count_in)[3], const int64_t (&stride_in)[3]) {
+    __int128 n[3] = {1, 1, 1}, s[3] = {0, 0, 0};
+    int m = 0;
+    for (int i = 0; i < 3; i++) {
+        if (count_in[i] <= 1) continue;
+        __int128 x = stride_in[i];
+        x = x < 0 ? -x : x;
+        if (x < block) return false;
+        int at = m++;
+        for (; at > 0 && s[at - 1] > x; at--) { s[at] = s[at - 1]; n[at] = n[at - 1]; }
+        s[at] = x; n[at] = count_in[i];
+    }
+    __int128 reach = block;
+    bool nested = true;
+    for (int i = 0; i < m; i++) {
+        nested &= s[i] >= reach;
+        reach += s[i] * (n[i] - 1);
+    }
+    if (nested) return true;
+    for (__int128 k = 0; k < n[2]; k++)
+        for (__int128 j = k ? 1 - n[1] : 0; j < n[1]; j++) {
+            if (j == 0 && k == 0) continue;                // one direction alone: its stride clears a block
+            const __int128 d = j * s[1] + k * s[2];
+            for (__int128 i = -d / s[0] - 1; i <= -d / s[0] + 1; i++) {
+                if (i <= -n[0] || i >= n[0]) continue;
+                const __int128 gap = d + i * s[0];
+                if (gap < block && gap > -(__int128)block) return false;
+            }
+        }
+    return true;
+}
+
 // The programmatic-dependent launch that the decode kernels use: the kernel waits on the device (grid_dependency_wait)
 // before it touches memory.
 template <typename... P, typename... A>

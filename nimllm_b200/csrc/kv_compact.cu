@@ -28,6 +28,19 @@ struct AcceptParams {
     int elem, row16;          // bytes per element, 16-byte pieces per row
 };
 
+// Both operators move rows within their blocks, a block at a time: blocks that overlap are refused.  With kv_off the host does not know
+// how far the sequences lie apart.
+int check_apart(const char *who, const CacheRows &rows, int n_layer, int64_t layer_stride, int batch, int n_kv_head) {
+    if (rows.table) {
+        if (n_layer > 1 && (layer_stride < 0 ? -layer_stride : layer_stride) < rows.n_pages * rows.page_stride)
+            return fail(NIMLLM_ERR_ARG, "%s: layer_stride %lld: the pages of two layers overlap", who, (long long)layer_stride);
+        return NIMLLM_OK;
+    }
+    if (blocks_apart((int64_t)rows.cap * rows.D, {n_layer, rows.kv_off ? 1 : batch, n_kv_head}, {layer_stride, rows.seq_stride, rows.head_stride})) return NIMLLM_OK;
+    return fail(NIMLLM_ERR_ARG, "%s: layer_stride %lld, seq_stride %lld, head_stride %lld: blocks of max_seq rows overlap", who, (long long)layer_stride,
+                (long long)rows.seq_stride, (long long)rows.head_stride);
+}
+
 // The usable length of a path: it ends before the first entry that is not a draft of this tree or does not lie behind its
 // predecessor.  Every thread of the block gets it; s_path holds the entries.
 __device__ __forceinline__ int path_length(const AcceptParams &p, int b, int len, int *s_path, int *s_m) {
@@ -104,6 +117,7 @@ int kv_accept(const char *who, const CacheRows &rows, void *k, void *v, int cach
     const int elem = (int)dtype_size(cache_dtype);
     if (head_dim <= 0 || head_dim * elem % 16 != 0) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: head_dim %d: rows must be a multiple of 16 bytes", who, head_dim);
     if (layer_stride * elem % 16 != 0) return fail(NIMLLM_ERR_ARG, "%s: layer_stride must be a multiple of 16 bytes", who);
+    if (int rc = check_apart(who, rows, n_layer, layer_stride, batch, n_kv_head)) return rc;
     AcceptParams p;
     p.k = (unsigned char *)k; p.v = (unsigned char *)v; p.rows = rows; p.layer_bytes = layer_stride * elem;
     p.path = path; p.n_path = n_path; p.seq_len = seq_len; p.new_len = new_len == seq_len ? nullptr : new_len;
@@ -366,6 +380,7 @@ int kv_evict(const char *who, const CacheRows &rows, void *k, void *v, int cache
     if ((int64_t)batch * n_kv_head > 0x7fffffff) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: too many (sequence, KV head) pairs", who);
     const int elem = (int)dtype_size(cache_dtype);
     if (head_dim <= 0 || head_dim * elem % 16 != 0) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: head_dim %d: rows must be a multiple of 16 bytes", who, head_dim);
+    if (int rc = check_apart(who, rows, 1, 0, batch, n_kv_head)) return rc;
     EvictParams p;
     p.k = (unsigned char *)k; p.v = (unsigned char *)v; p.rows = rows; p.score = score; p.score_rows = score_rows; p.seq_len = seq_len;
     p.new_len = new_len == seq_len ? nullptr : new_len; p.kept = kept; p.max_len = max_len; p.keep = keep; p.n_sink = n_sink;

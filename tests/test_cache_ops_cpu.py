@@ -117,6 +117,29 @@ def test_accept_refusals():
     refused(go(D=60), 2, "16 bytes")
 
 
+@pytest.mark.parametrize("change,word", [
+    (dict(ls=0), "layer_stride 0"), (dict(ls=8192 - 8), "overlap"), (dict(ls=-(8192 - 8)), "overlap"), (dict(hs=0), "head_stride 0"), (dict(hs=8192 - 8), "overlap"),
+    (dict(ss=0, B=2), "seq_stride 0"), (dict(ss=8192, B=2, hs=8192), "overlap"),             # sequence 1, head 0 is sequence 0, head 1
+    (dict(ls=3 * 8192, hs=8192, Hkv=4), "overlap"), (dict(ls=5 * 8192, ss=2 * 8192, hs=8192, B=4), "overlap"), (dict(ls=8192, off=P), "overlap")])
+def test_accept_refuses_blocks_that_overlap(change, word):
+    a = dict(k=P, v=P, ct=1, L=2, ls=1 << 20, off=None, ss=65536, hs=16384, cap=128, path=P, mp=4, np=P, len=P, new=P, n=8, B=1, Hkv=2, D=64, st=None)
+    a.update({**dict(hs=8192), **change})
+    refused(L.nimllm_kv_accept(*a.values()), 1, word)
+
+
+@pytest.mark.parametrize("ls", [0, 9 * 2 * 32 * 64 - 8])
+def test_accept_refuses_pages_of_layers_that_overlap(ls):
+    refused(L.nimllm_kv_accept_paged(P, P, 1, 2, ls, P, 4, 32, 9, P, 4, P, P, P, 8, 1, 2, 64, None), 1, "overlap")
+
+
+@pytest.mark.parametrize("change", [dict(hs=0), dict(ss=0, B=2), dict(ss=8192, hs=8192, B=2), dict(hs=4096, off=P)])
+def test_evict_refuses_blocks_that_overlap(change):
+    a = dict(k=P, v=P, ct=1, off=None, ss=65536, hs=16384, cap=128, score=P, rows=128, len=P, max_len=128, keep=64, sink=4, recent=8, kept=P, new=P,
+             B=1, Hkv=2, D=64, st=None)
+    a.update(change)
+    refused(L.nimllm_kv_evict(*a.values()), 1, "overlap")
+
+
 def test_evict_refusals():
     f = L.nimllm_kv_evict
 
