@@ -52,6 +52,9 @@ __device__ __forceinline__ int64_t tree_out_row(const TreeParams &p, int b, int 
     return ((int64_t)b * p.n + i) * p.Hq + kvh * p.G + (qr - i * p.G);
 }
 
+// 1 / l for the sum l of a softmax: 0 for a row that attends nothing, and no number where a score that it attends is none or infinite
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : (l < INFINITY ? 1.f / l : NAN); }
+
 // the kernels for bf16 caches (tree_wide_tc.cu, tree_narrow_tc.cu) and for fp32 caches (tree_f32.cu)
 size_t tree_tc_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim);
 size_t tree_f32_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, int max_total);

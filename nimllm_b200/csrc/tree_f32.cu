@@ -193,12 +193,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) tree_f32_narrow_kernel(TreePar
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
                 const float2 ml = s_ml[w * RC + r];
-                const float f = ml.y > 0.f ? ex2(ml.x - M) : 0.f;
+                const float f = ml.y != 0.f ? ex2(ml.x - M) : 0.f;
                 L += ml.y * f;
                 const float4 x = *reinterpret_cast<const float4 *>(s_acc + (w * RC + r) * D + col);
                 o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
             }
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const float inv = inverse_sum(L);
             o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
             const int64_t orow = tree_out_row(p, sg.b, sg.kvh, r);
             const float m = M == kUnset ? -INFINITY : M;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(128) tree_f32_tiled_kernel(TreeParams p) {
     for (int i = 0; i < TI; i++) {
         const int qr = q0 + rg + 16 * i;
         if (qr >= R) continue;
-        const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+        const float inv = inverse_sum(l[i]);
         const int64_t orow = tree_out_row(p, b, kvh, qr);
         float *rec = n_chunks > 1 ? p.recs + ((int64_t)chunk * p.B * p.n * p.Hq + orow) * W : nullptr;
 #pragma unroll

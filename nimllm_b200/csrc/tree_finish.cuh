@@ -56,12 +56,13 @@ template <int D> __device__ __forceinline__ Pieces chunk_pieces(const TreeParams
     return x;
 }
 
-// maximum (natural units) and, relative to it, the sum of a row's pieces, in every lane
+// maximum (natural units) and, relative to it, the sum of a row's pieces, in every lane.  A piece is empty when its sum is zero; one whose
+// sum is NaN counts, so that the row has no number either.
 template <int D> __device__ __forceinline__ void pieces_stats(const Pieces &x, int lane, float &M, float &L) {
     M = -INFINITY;
     for (int i = lane; i < x.n; i += 32) {
         const float2 ml = *reinterpret_cast<const float2 *>(x.rec(i) + D / 4 * x.col);
-        if (ml.y > 0.f) M = fmaxf(M, ml.x);
+        if (ml.y != 0.f) M = fmaxf(M, ml.x);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
@@ -69,7 +70,7 @@ template <int D> __device__ __forceinline__ void pieces_stats(const Pieces &x, i
     L = 0.f;
     for (int i = lane; i < x.n; i += 32) {
         const float2 ml = *reinterpret_cast<const float2 *>(x.rec(i) + D / 4 * x.col);
-        if (ml.y > 0.f) L += ml.y * ex2((ml.x - safe) * kLog2e);
+        if (ml.y != 0.f) L += ml.y * ex2((ml.x - safe) * kLog2e);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
@@ -93,18 +94,18 @@ __device__ __forceinline__ void join_rows(const TreeParams &p, const Pieces &x, 
         const unsigned mask = 0xffu << (threadIdx.x & 24);
         float M = -INFINITY, L = 0.f;
         for (int i = sub; i < x.n; i += kLanes)
-            if (ml[i].y > 0.f) M = fmaxf(M, ml[i].x);
+            if (ml[i].y != 0.f) M = fmaxf(M, ml[i].x);
 #pragma unroll
         for (int off = kLanes / 2; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(mask, M, off));
         const float safe = M == -INFINITY ? 0.f : M;
         for (int i = sub; i < x.n; i += kLanes) {
-            const float w = ml[i].y > 0.f ? ml[i].y * ex2((ml[i].x - safe) * kLog2e) : 0.f;
+            const float w = ml[i].y != 0.f ? ml[i].y * ex2((ml[i].x - safe) * kLog2e) : 0.f;
             ml[i].x = w;
             L += w;
         }
 #pragma unroll
         for (int off = kLanes / 2; off > 0; off >>= 1) L += __shfl_xor_sync(mask, L, off);
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = inverse_sum(L);
         for (int i = sub; i < x.n; i += kLanes) ml[i].x *= inv;
         if (sub == 0 && p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + out_row(r) * W + D) = make_float4(M, L, 0.f, 0.f);
     }
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kFinishThreads, 4) tree_finish_kernel(TreePara
         const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g, len, p.G) : chunk_pieces<D>(p, h0 + g, len);
         float M, L;
         pieces_stats<D>(pc, lane, M, L);
-        if (lane == 0) s_stat[g] = make_float2(M * kLog2e, L > 0.f ? 1.f / L : 0.f);
+        if (lane == 0) s_stat[g] = make_float2(M * kLog2e, inverse_sum(L));
     }
     __syncthreads();
     for (; row < min(len, r0 + kScoreRows); row += 4 * kFinishThreads) {

@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_narrow_kernel(TreeParams p, 
                 const float s1 = (sb.wsum[1][0][r] + sb.wsum[1][1][r]) + (sb.wsum[1][2][r] + sb.wsum[1][3][r]);
                 const float M = fmaxf(r0, r1), m = M == kUnset ? -INFINITY : M;
                 const float f0 = ex2(r0 - M), f1 = ex2(r1 - M);
-                const float L = s0 * f0 + s1 * f1, inv = L > 0.f ? 1.f / L : 0.f;
+                const float L = s0 * f0 + s1 * f1, inv = inverse_sum(L);
                 const int64_t orow = tree_out_row(p, sg.b, sg.kvh, r);
                 sb.join[r] = make_float2(f0 * inv, f1 * inv);
                 sb.orow[r] = orow;

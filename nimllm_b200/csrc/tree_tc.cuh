@@ -168,7 +168,7 @@ __device__ __forceinline__ void store_row8(const TreeParams &p, int64_t orow, in
 template <int D>
 __device__ __forceinline__ void store_row_stats(const TreeParams &p, int64_t orow, float m, float l) {
     if (p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + D) = make_float4(m * kLn2, l, 0.f, 0.f);
-    if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(m, l > 0.f ? 1.f / l : 0.f);
+    if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(m, inverse_sum(l));
 }
 
 // a row that was cut has no statistics yet: the score blocks join its pieces themselves

@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                 if (lane == 0) mbar_arrive(&sb.x_ready);
                 continue;
             }
-            float m = ref, f0 = l > 0.f ? 1.f : 0.f, f1 = 0.f;
+            float m = ref, f0 = l != 0.f ? 1.f : 0.f, f1 = 0.f;      // 0: the group has nothing; a sum that is NaN counts
             if (!SPLIT) {
                 if (!(ok = wait(&sb.x_ready, seg & 1))) break;
                 tc_fence_after();
@@ -553,18 +553,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                 f0 = ex2(ref - m);
                 f1 = ex2(o.x - m);
                 const float sum = l * f0 + o.y * f1;
-                f0 = l > 0.f ? f0 : 0.f;
-                f1 = o.y > 0.f ? f1 : 0.f;
+                f0 = l != 0.f ? f0 : 0.f;
+                f1 = o.y != 0.f ? f1 : 0.f;
                 l = sum;
             }
             if (busy) {
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const float inv = inverse_sum(l);                  // may be NaN: a group that has nothing stays at 0
                 f0 *= inv;
-                f1 *= inv;
+                if (!SPLIT) f1 = f1 != 0.f ? f1 * inv : 0.f;
                 m = m == kUnset ? -INFINITY : m;
                 const int64_t orow = tree_out_row(p, sg.b, sg.kvh, qr);
                 float *rec = sg.flags & 1 ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * a.rec_rows * W + ((SPLIT ? g * kRows : 0) + row) * 4;
-                const bool any1 = __any_sync(0xffffffffu, f1 != 0.f);
+                const bool any1 = !SPLIT && __any_sync(0xffffffffu, f1 != 0.f);      // split rows have no second O: no columns behind group 1's
 #pragma unroll
                 for (int y0 = 0; y0 < D; y0 += 16) {
                     float v[16];
