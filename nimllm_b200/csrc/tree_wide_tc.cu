@@ -21,6 +21,8 @@
 // registers every few tiles: thousands of rows added up by the tensor core would lose what 32-bit results promise.  For bf16 results
 // P is rounded to bf16 like the result itself (the sum is taken of the rounded values, so that a single large weight stays exact);
 // a second term would make this kernel a third slower, whose tensor pipe has 24 products for every 256 query rows x 64 cached ones.
+// That is the precision of more than 32 query rows only: 17 - 32 rows of an fp32 q with heads of 128, which the narrow kernel does not
+// take, have two terms (2^-17 left) as its rows have: 32 sequences of 2 - 4 K rows, 20 query rows, 140 us, with one term 128.
 //
 // Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 152 us (160 without the
 // rows' policy of leaving L2 first, which keeps records, Q and code there).  The rows' bytes at the measured peak of HBM are 65 us, the
@@ -156,7 +158,7 @@ __device__ __forceinline__ void hide32(float *x, uint32_t vis) {
         if (!((vis >> y) & 1)) x[y] = -INFINITY;
 }
 
-// NQ, NP: terms of q (1, 3) and of P (1, 3); SPLIT: 256 query rows a tile, half of them per group (else 128, the tiles in turn)
+// NQ, NP: terms of q (1, 3) and of P (1, 2, 3); SPLIT: 256 query rows a tile, half of them per group (else 128, the tiles in turn)
 template <int D, int NQ, int NP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, TcArgs a) {
     constexpr int RPT = SPLIT ? 2 * kRows : kRows;
@@ -663,6 +665,7 @@ cudaError_t launch_d(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     cudaError_t e;
     if (narrow) e = launch_tree_narrow(p, a, D, st);
     else if (a.q_terms == 1) e = a.p_terms == 2 ? launch_wide<D, 1, 1>(p, a, st) : launch_wide<D, 1, 3>(p, a, st);
+    else if (D == 128 && a.p_terms == 2 && R <= kNarrowRows) e = launch_wide<128, 3, 2>(p, a, st);     // rows that the narrow kernel leaves
     else e = a.p_terms == 2 ? launch_wide<D, 3, 1>(p, a, st) : launch_wide<D, 3, 3>(p, a, st);
     if (e != cudaSuccess) return e;
     FinishArgs f = {};

@@ -6,7 +6,7 @@ import torch
 
 import cache_util as U
 from nimllm_b200 import attention as A
-from test_gpu_decode_tree import _scored_case
+from test_gpu_decode_tree import _scored_case, _tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,10 @@ def test_an_infinite_score_leaves_no_number(row, cache_dtype, Hq):
     G = Hq // Hkv
     assert torch.isnan(out[:G]).all() and torch.isnan(score[0, 0]).all()
     assert torch.isfinite(out[G:]).all() and torch.isfinite(score[0, 1]).all()
+
+
+@pytest.mark.parametrize("n,Hq,Hkv", [(5, 8, 2), (8, 4, 1), (17, 2, 2), (32, 1, 1)])
+def test_weights_of_17_to_32_query_rows_keep_32_bits(n, Hq, Hkv):
+    for seed in range(55, 60):
+        _tree_case(seed, [100, 0, 37, 500], n, Hq, Hkv, 128, F, H, H, 0, "tree")
+        _tree_case(seed, [60, 3000], n, Hq, Hkv, 128, F, H, H, 64, "chain", ragged=False)
