@@ -52,8 +52,8 @@ __device__ __forceinline__ int64_t tree_out_row(const TreeParams &p, int b, int 
     return ((int64_t)b * p.n + i) * p.Hq + kvh * p.G + (qr - i * p.G);
 }
 
-// 1 / l for the sum l of a softmax: 0 for a row that attends nothing, and no number where a score that it attends is none or infinite
-__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : (l < INFINITY ? 1.f / l : NAN); }
+// 1 / l for the sum l of a softmax, 0 for a row that attends nothing.  NaN stays NaN, and an infinite sum times the 0 that it gives.
+__device__ __forceinline__ float inverse_sum(float l) { return l != 0.f ? 1.f / l : 0.f; }
 
 // the kernels for bf16 caches (tree_wide_tc.cu, tree_narrow_tc.cu) and for fp32 caches (tree_f32.cu)
 size_t tree_tc_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim);

@@ -22,7 +22,7 @@
 // P is rounded to bf16 like the result itself (the sum is taken of the rounded values, so that a single large weight stays exact);
 // a second term would make this kernel a third slower, whose tensor pipe has 24 products for every 256 query rows x 64 cached ones.
 // That is the precision of more than 32 query rows only: 17 - 32 rows of an fp32 q with heads of 128, which the narrow kernel does not
-// take, have two terms (2^-17 left) as its rows have: 32 sequences of 2 - 4 K rows, 20 query rows, 140 us, with one term 128.
+// take, have two terms (2^-17 left) as its rows have: 32 sequences of 2 - 4 K rows, 20 query rows, 130 us.
 //
 // Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 152 us (160 without the
 // rows' policy of leaving L2 first, which keeps records, Q and code there).  The rows' bytes at the measured peak of HBM are 65 us, the
@@ -567,7 +567,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_wide_kernel(TreeParams p, Tc
                 const int64_t orow = tree_out_row(p, sg.b, sg.kvh, qr);
                 float *rec = sg.flags & 1 ? nullptr : p.recs + ((int64_t)blockIdx.x * 2 + (sg.flags >> 1)) * a.rec_rows * W + ((SPLIT ? g * kRows : 0) + row) * 4;
                 const bool any1 = !SPLIT && __any_sync(0xffffffffu, f1 != 0.f);      // split rows have no second O: no columns behind group 1's
-#pragma unroll
+                // O in TMEM: rolled, for less code to fetch once a segment (48 rows over 2 - 4 K 106 -> 96 us); O in registers has fixed names
+#pragma unroll (NP == 3 ? D / 16 : 1)
                 for (int y0 = 0; y0 < D; y0 += 16) {
                     float v[16];
                     if constexpr (NP == 3) {
