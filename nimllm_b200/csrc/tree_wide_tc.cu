@@ -22,7 +22,9 @@
 // P is rounded to bf16 like the result itself (the sum is taken of the rounded values, so that a single large weight stays exact);
 // a second term would make this kernel a third slower, whose tensor pipe has 24 products for every 256 query rows x 64 cached ones.
 // That is the precision of more than 32 query rows only: 17 - 32 rows of an fp32 q with heads of 128, which the narrow kernel does not
-// take, have two terms (2^-17 left) as its rows have: 32 sequences of 2 - 4 K rows, 20 query rows, 130 us.
+// take, have two terms (2^-17 left) as its rows have: 32 sequences of 2 - 4 K rows, 20 query rows, 130 us.  Scored decode has two as
+// well, so that l is the sum of the weights themselves, which the scores are divided by (32 sequences of 2 - 4 K rows, 40 heads of 128:
+// 102 us, with one term 100).
 //
 // Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 152 us (160 without the
 // rows' policy of leaving L2 first, which keeps records, Q and code there).  The rows' bytes at the measured peak of HBM are 65 us, the
@@ -664,10 +666,12 @@ cudaError_t launch_d(const TreeParams &p, TcArgs &a, cudaStream_t st) {
     const int R = p.n * p.G;
     const bool narrow = tree_narrow_takes(R, a.q_terms, a.p_terms, D);
     cudaError_t e;
+    // terms of P: three for 32-bit results, else one where its rounding is no larger than the result's.  Two for rows that the narrow kernel
+    // leaves, and where scores are kept: their softmax has the same sum l, which one term would have to round with P
+    const int np = a.p_terms == 3 ? 3 : (R <= kNarrowRows || p.score ? 2 : 1);
     if (narrow) e = launch_tree_narrow(p, a, D, st);
-    else if (a.q_terms == 1) e = a.p_terms == 2 ? launch_wide<D, 1, 1>(p, a, st) : launch_wide<D, 1, 3>(p, a, st);
-    else if (D == 128 && a.p_terms == 2 && R <= kNarrowRows) e = launch_wide<128, 3, 2>(p, a, st);     // rows that the narrow kernel leaves
-    else e = a.p_terms == 2 ? launch_wide<D, 3, 1>(p, a, st) : launch_wide<D, 3, 3>(p, a, st);
+    else if (a.q_terms == 1) e = np == 1 ? launch_wide<D, 1, 1>(p, a, st) : (np == 2 ? launch_wide<D, 1, 2>(p, a, st) : launch_wide<D, 1, 3>(p, a, st));
+    else e = np == 1 ? launch_wide<D, 3, 1>(p, a, st) : (np == 2 ? launch_wide<D, 3, 2>(p, a, st) : launch_wide<D, 3, 3>(p, a, st));
     if (e != cudaSuccess) return e;
     FinishArgs f = {};
     f.tc = a; f.rpt = rows_per_tile(R, a.q_terms, a.p_terms, D); f.tile = narrow ? kNarrowTile : kTile; f.workers = sm_count(); f.by_col = !narrow;

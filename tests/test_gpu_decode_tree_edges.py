@@ -94,3 +94,9 @@ def test_weights_of_17_to_32_query_rows_keep_32_bits(n, Hq, Hkv):
     for seed in range(55, 60):
         _tree_case(seed, [100, 0, 37, 500], n, Hq, Hkv, 128, F, H, H, 0, "tree")
         _tree_case(seed, [60, 3000], n, Hq, Hkv, 128, F, H, H, 64, "chain", ragged=False)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,q_dtype", [(20, 1, 128, F), (40, 1, 128, H), (40, 1, 64, H), (40, 1, 64, F), (96, 2, 128, F), (160, 1, 128, F), (300, 1, 64, H)])
+def test_scores_beside_bf16_results_keep_32_bits(Hq, Hkv, D, q_dtype):
+    _scored_case(61, [130, 5, 64, 700, 0, 3000], Hq, Hkv, D, q_dtype, H, H, 0, 1.0)
+    _scored_case(62, [100, 257], Hq, Hkv, D, q_dtype, H, H, 32, 0.5)
