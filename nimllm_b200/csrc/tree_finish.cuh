@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kFinishThreads, 4) tree_finish_kernel(TreePara
         const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g, len, p.G) : chunk_pieces<D>(p, h0 + g, len);
         float M, L;
         pieces_stats<D>(pc, lane, M, L);
-        if (lane == 0) s_stat[g] = make_float2(M * kLog2e + (L - L), inverse_sum(L));
+        if (lane == 0) s_stat[g] = score_stats(M * kLog2e, L);
     }
     __syncthreads();
     for (; row < min(len, r0 + kScoreRows); row += 4 * kFinishThreads) {

@@ -100,3 +100,18 @@ def test_weights_of_17_to_32_query_rows_keep_32_bits(n, Hq, Hkv):
 def test_scores_beside_bf16_results_keep_32_bits(Hq, Hkv, D, q_dtype):
     _scored_case(61, [130, 5, 64, 700, 0, 3000], Hq, Hkv, D, q_dtype, H, H, 0, 1.0)
     _scored_case(62, [100, 257], Hq, Hkv, D, q_dtype, H, H, 32, 0.5)
+
+
+@pytest.mark.parametrize("Hq", [4, 24, 80])
+@pytest.mark.parametrize("cache_dtype", [F, H])
+def test_scores_of_rows_that_count_as_hidden(cache_dtype, Hq):
+    """Scaled scores below -1e30 everywhere: no NaN comes out of a sum that has nothing in it."""
+    Hkv, D, L = 2, 64, 300
+    k = -torch.ones(1, Hkv, L, D, dtype=cache_dtype, device="cuda")
+    v = torch.ones_like(k)
+    score = torch.full((1, Hkv, L), 3.0, device="cuda")
+    out = A.decode_scored(torch.ones(1, Hq * D, device="cuda"), k, v, score, n_head=Hq, n_kv_head=Hkv, head_dim=D, max_len=L, max_seq=L, scale=1e30,
+                          seq_stride=Hkv * L * D, head_stride=L * D, decay=0.5)
+    assert torch.isfinite(out).all() and torch.isfinite(score).all()
+    added = (score - 1.5).sum(-1)                          # nothing, or the equal weights of a softmax
+    assert ((added == 0) | ((added - Hq // Hkv).abs() < 1e-3)).all()
