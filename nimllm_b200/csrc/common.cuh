@@ -123,6 +123,21 @@ __device__ __forceinline__ void peer_push_publish(const PeerPush &px, unsigned i
 inline size_t dtype_size(int dtype) { return dtype == NIMLLM_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == NIMLLM_F32 || dtype == NIMLLM_BF16; }
 
+// Reads (and clears) a sticky status word of the current device once everything launched on it has ended, on non-blocking streams too:
+// a copy alone waits for the blocking ones only.  NIMLLM_OK or the status with its message set.
+template <typename Word> int read_status_word(const char *who, Word &word, int reset, int *out) {
+    int st = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&st, word, sizeof(int));
+    if (e == cudaSuccess && reset && st != 0) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(word, &zero, sizeof(int));
+    }
+    if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    *out = st;
+    return NIMLLM_OK;
+}
+
 int sm_count();  // multiprocessors of the current device (cached per device)
 
 // ---- kernel launchers implemented in the .cu files (device pointers, validated args) ----

@@ -1040,13 +1040,8 @@ int nimllm_qkv_rope_append(const float *x_norm, const void *wq, const void *wk, 
 
 int nimllm_matvec_status(int reset) {
     int st = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&st, g_matvec_status, sizeof(int));
-    if (e == cudaSuccess && reset && st != 0) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(g_matvec_status, &zero, sizeof(int));
-    }
-    if (e != cudaSuccess) return -fail(NIMLLM_ERR_CUDA, "matvec_status: %s", cudaGetErrorString(e));
-    return st;
+    const int rc = read_status_word("matvec_status", g_matvec_status, reset, &st);
+    return rc ? -rc : st;
 }
 
 /* src/kernels.cu:996-1003 and :1053-1059: y[rows] = A[rows, cols] x[cols], legacy default stream, void */

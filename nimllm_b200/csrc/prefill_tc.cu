@@ -623,15 +623,7 @@ int launch_prefill_tc(void *q, const void *k, const void *v, void *out, float *l
 // Reads (and with reset != 0 clears) the sticky status word of the current device.  Synchronises
 // the device: call it where the host waits for results anyway.
 int prefill_tc_status(int reset, int *status_out) {
-    int st = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&st, g_prefill_status, sizeof(int));
-    if (e == cudaSuccess && reset && st != 0) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(g_prefill_status, &zero, sizeof(int));
-    }
-    if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "attn_prefill_status: %s", cudaGetErrorString(e));
-    *status_out = st;
-    return NIMLLM_OK;
+    return read_status_word("attn_prefill_status", g_prefill_status, reset, status_out);
 }
 
 }  // namespace nimllm

@@ -636,15 +636,7 @@ cudaError_t launch_tree_narrow(const TreeParams &p, TcArgs &a, int head_dim, cud
 }
 
 int tree_narrow_status(int reset, int *status_out) {
-    int st = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&st, g_narrow_status, sizeof(int));
-    if (e == cudaSuccess && reset && st != 0) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(g_narrow_status, &zero, sizeof(int));
-    }
-    if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "attn_decode_tree_status: %s", cudaGetErrorString(e));
-    *status_out = st;
-    return NIMLLM_OK;
+    return read_status_word("attn_decode_tree_status", g_narrow_status, reset, status_out);
 }
 
 }  // namespace treetc

@@ -704,26 +704,11 @@ int launch_tree_tc(const char *who, TreeParams &p, int head_dim, void *workspace
     return NIMLLM_OK;
 }
 
-namespace treetc {
-// Reads (and clears) a sticky word of the current device.
-template <typename T> static int read_status(T &word, int reset, int *out) {
-    int st = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&st, word, sizeof(int));
-    if (e == cudaSuccess && reset && st != 0) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbol(word, &zero, sizeof(int));
-    }
-    if (e != cudaSuccess) return fail(NIMLLM_ERR_CUDA, "attn_decode_tree_status: %s", cudaGetErrorString(e));
-    *out = st;
-    return NIMLLM_OK;
-}
-
-}  // namespace treetc
 }  // namespace nimllm
 
 extern "C" int nimllm_attn_decode_tree_status(int reset) {
     int wide = 0, narrow = 0;
-    int rc = nimllm::treetc::read_status(nimllm::treetc::g_wide_status, reset, &wide);
+    int rc = nimllm::read_status_word("attn_decode_tree_status", nimllm::treetc::g_wide_status, reset, &wide);
     if (!rc) rc = nimllm::treetc::tree_narrow_status(reset, &narrow);
     return rc ? -rc : (wide | narrow);
 }
