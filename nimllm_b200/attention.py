@@ -387,12 +387,15 @@ def rope_append_at(q, k_new, v_new, cos, sin, *, n_head, n_kv_head, head_dim, la
     return q_out, k_out
 
 
-def _pages(index, k_pages, v_pages, page_table, batch, n_kv_head, head_dim, layers=1):
-    """(pointers of K, V and the table, max_pages, page_rows, n_pages) of pages [(layers,) n_pages, Hkv, page_rows, D], checked
-    against the heads and the table."""
+def _pages(index, k_pages, v_pages, page_table, batch, n_kv_head, head_dim, layers=None):
+    """(pointers of K, V and the table, max_pages, page_rows, n_pages) of pages [n_pages, Hkv, page_rows, D], checked against the
+    heads and the table; a layer axis in front only for a call that says how many layers it means (or where it has one entry)."""
     shape = k_pages.shape
-    n_pages, heads, page_rows, width = shape[-4:]
-    if len(shape) not in (4, 5) or heads != n_kv_head or width != head_dim or v_pages.shape != shape:
+    if layers is None and len(shape) == 5 and shape[0] != 1:
+        raise _lib.NimllmAttnError(f"pages {tuple(shape)}: this call works on one layer, give pages[layer]")
+    layers = layers or 1
+    n_pages, heads, page_rows, width = shape[-4:] if len(shape) in (4, 5) else (0, 0, 0, 0)
+    if heads != n_kv_head or width != head_dim or v_pages.shape != shape:
         raise _lib.NimllmAttnError(f"pages {tuple(shape)} / {tuple(v_pages.shape)}: [n_pages, {n_kv_head}, page_rows, {head_dim}] expected")
     if (shape[0] if len(shape) == 5 else 1) < layers:
         raise _lib.NimllmAttnError(f"pages {tuple(shape)}: {layers} layers expected")

@@ -166,6 +166,40 @@ def test_python_checks_shapes_before_anything_runs():
         A.rope_append_at(t, t, t, None, None, n_head=4, n_kv_head=4, head_dim=64)
 
 
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The wrappers' own checks, with tensors on the CPU and a library that must not be reached."""
+    monkeypatch.setattr(A, "_on", lambda t: (-1, A._here))
+
+    class NotReached:
+        def __getattr__(self, name):
+            raise AssertionError(f"{name} was called")
+    monkeypatch.setattr(A, "lib", NotReached)
+
+
+def test_pages_of_several_layers_are_refused_by_calls_for_one(on_cpu):
+    pages, table = torch.zeros(3, 8, 2, 32, 64), torch.zeros(1, 4, dtype=torch.int32)
+    q, kw = torch.zeros(1, 2, 256), dict(n_head=4, n_kv_head=2, head_dim=64)
+    kv = torch.zeros(1, 2, 128)
+    calls = [lambda p: A.decode_tree_paged(q, p, p, table, max_len=10, **kw),
+             lambda p: A.decode_scored_paged(q[:, 0], p, p, table, torch.zeros(1, 2, 10), max_len=10, **kw),
+             lambda p: A.rope_append_at_paged(q, kv, kv, None, None, p, p, table, **kw),
+             lambda p: A.kv_evict_paged(p, p, table, torch.zeros(1, 2, 10), None, keep=4, n_kv_head=2, head_dim=64, max_len=10)]
+    for call in calls:
+        with pytest.raises(_lib.NimllmAttnError, match="one layer"):
+            call(pages)
+        for one in (pages[0], pages[:1]):                  # as before
+            with pytest.raises(AssertionError, match="was called"):
+                call(one)
+        with pytest.raises(_lib.NimllmAttnError, match="expected"):
+            call(pages[0, 0])
+    ints = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(_lib.NimllmAttnError, match="4 layers expected"):
+        A.kv_accept_paged(pages, pages, table, ints.view(1, 1), ints, ints, n_draft=1, n_kv_head=2, head_dim=64, n_layer=4)
+    with pytest.raises(AssertionError, match="was called"):
+        A.kv_accept_paged(pages, pages, table, ints.view(1, 1), ints, ints, n_draft=1, n_kv_head=2, head_dim=64, n_layer=2)
+
+
 def _freqs(rot, base):
     return base ** (-2.0 * np.arange(rot // 2) / rot)
 
