@@ -273,7 +273,9 @@ def _small(name, t, least):
 
 
 def _block_end(batch, n_kv_head, head_dim, seq_stride, head_stride, max_seq, layers=0, layer_stride=0):
-    """Elements that the blocks of a contiguous cache without kv_off reach over."""
+    """Elements that the blocks of a contiguous cache without kv_off reach over, from its first element on."""
+    if (seq_stride < 0 and batch > 1) or (head_stride < 0 and n_kv_head > 1) or (layer_stride < 0 and layers > 1):
+        raise _lib.NimllmAttnError(f"seq_stride {seq_stride}, head_stride {head_stride}, layer_stride {layer_stride}: a cache starts with its first block")
     return (layers - 1 if layers > 1 else 0) * layer_stride + (batch - 1) * seq_stride + (n_kv_head - 1) * head_stride + max_seq * head_dim
 
 

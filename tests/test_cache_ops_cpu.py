@@ -200,6 +200,24 @@ def test_pages_of_several_layers_are_refused_by_calls_for_one(on_cpu):
         A.kv_accept_paged(pages, pages, table, ints.view(1, 1), ints, ints, n_draft=1, n_kv_head=2, head_dim=64, n_layer=2)
 
 
+@pytest.mark.parametrize("strides", [dict(seq_stride=-8192, head_stride=4096), dict(seq_stride=8192, head_stride=-4096)])
+def test_blocks_in_front_of_a_cache_are_refused(on_cpu, strides):
+    c, q, kv = torch.zeros(3 * 8192), torch.zeros(3, 2, 256), torch.zeros(3, 2, 128)
+    score, ints = torch.zeros(3, 2, 64), torch.zeros(3, dtype=torch.int32)
+    heads, kv_heads, where = dict(n_head=4, n_kv_head=2, head_dim=64), dict(n_kv_head=2, head_dim=64), dict(max_seq=64)
+    calls = [lambda **w: A.decode_tree(q, c, c, max_len=10, **heads, **w), lambda **w: A.decode_scored(q[:, 0].contiguous(), c, c, score, max_len=10, **heads, **w),
+             lambda **w: A.rope_append_at(q, kv, kv, None, None, k_cache=c, v_cache=c, **heads, **w),
+             lambda **w: A.kv_accept(c, c, ints.view(3, 1), ints, ints, n_draft=1, **kv_heads, **w),
+             lambda **w: A.kv_evict(c, c, score, None, keep=4, max_len=64, **kv_heads, **w)]
+    for call in calls:
+        with pytest.raises(_lib.NimllmAttnError, match="first block"):
+            call(**strides, **where)
+        with pytest.raises(AssertionError, match="was called"):
+            call(seq_stride=8192, head_stride=4096, **where)
+    with pytest.raises(_lib.NimllmAttnError, match="first block"):
+        A.kv_accept(c, c, ints.view(3, 1), ints, ints, n_draft=1, n_layer=2, layer_stride=-3 * 8192, seq_stride=8192, head_stride=4096, **kv_heads, **where)
+
+
 def _freqs(rot, base):
     return base ** (-2.0 * np.arange(rot // 2) / rot)
 
