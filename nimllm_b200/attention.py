@@ -377,12 +377,14 @@ def rope_append_at(q, k_new, v_new, cos, sin, *, n_head, n_kv_head, head_dim, la
                                             k_out, want_k, k_cache is not None)
         kc = vc = off = None
         code = F32
+        if (k_cache is None) != (v_cache is None):
+            raise _lib.NimllmAttnError("give both k_cache and v_cache or neither")
         if k_cache is not None:
             kc, vc, off = _args(index, (None, k_cache.dtype, _I64), (k_cache, v_cache, kv_off))
             code = _code(k_cache)
-            if kv_off is None and v_cache is not None:
+            if kv_off is None:
                 _check_blocks(k_cache, v_cache, _block_end(B, n_kv_head, head_dim, seq_stride, head_stride, max_seq))
-            elif kv_off is not None and kv_off.numel() < B:
+            elif kv_off.numel() < B:
                 _small("kv_off", kv_off, B)
         check(lib().nimllm_rope_append_at(*head, first_row, kc, vc, code, off, seq_stride, head_stride, max_seq, B, n, n_kv_head, head_dim,
                                           _raw_stream(index)))

@@ -218,6 +218,13 @@ def test_blocks_in_front_of_a_cache_are_refused(on_cpu, strides):
         A.kv_accept(c, c, ints.view(3, 1), ints, ints, n_draft=1, n_layer=2, layer_stride=-3 * 8192, seq_stride=8192, head_stride=4096, **kv_heads, **where)
 
 
+def test_one_cache_of_two_is_refused(on_cpu):
+    kv, c, kw = torch.zeros(1, 2, 128), torch.zeros(8192), dict(n_head=4, n_kv_head=2, head_dim=64, head_stride=4096, max_seq=64)
+    for k_cache, v_cache in ((c, None), (None, c)):
+        with pytest.raises(_lib.NimllmAttnError, match="both"):
+            A.rope_append_at(None, kv, kv, None, None, k_cache=k_cache, v_cache=v_cache, **kw)
+
+
 def _freqs(rot, base):
     return base ** (-2.0 * np.arange(rot // 2) / rot)
 
