@@ -20,6 +20,11 @@ size_t record_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, i
 // whole tiles of the tensor-core kernels are written
 int64_t raw_rows(int max_len) { return ((int64_t)max_len + 127) / 128 * 128; }
 
+// what the launches' grids and 32-bit row numbers hold
+bool fits(int batch, int n, int n_head, int n_kv_head, int max_len) {
+    return batch <= 65535 && (int64_t)n_kv_head * (((int64_t)n * (n_head / n_kv_head) + 31) / 32) <= 65535 && max_len <= (1 << 30);
+}
+
 // q, shapes and the workspace of both entry points
 int tree_launch(const char *who, TreeParams &p, const void *workspace, size_t workspace_bytes, size_t need, int cache_dtype, int head_dim,
                 cudaStream_t st) {
@@ -46,7 +51,7 @@ int check_shape(const char *who, const void *q, int q_dtype, const void *out, in
     if (!dtype_ok(q_dtype) || !dtype_ok(out_dtype)) return fail(NIMLLM_ERR_ARG, "%s: unknown dtype", who);
     if (head_dim != 64 && head_dim != 128) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: head_dim %d (64 and 128 are built)", who, head_dim);
     if (n > kTreeMaxTokens) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: n %d > %d", who, n, kTreeMaxTokens);
-    if (batch > 65535 || (int64_t)n_kv_head * (((int64_t)n * (n_head / n_kv_head) + 31) / 32) > 65535 || max_len > (1 << 30))
+    if (!fits(batch, n, n_head, n_kv_head, max_len))
         return fail(NIMLLM_ERR_UNSUPPORTED, "%s: batch %d, n %d, Hq %d or max_len %d is too large", who, batch, n, n_head, max_len);
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)partials_out) & 15) return fail(NIMLLM_ERR_ARG, "%s: q and the outputs must be 16-byte aligned", who);
     return NIMLLM_OK;
@@ -93,7 +98,9 @@ using namespace nimllm;
 extern "C" {
 
 size_t nimllm_attn_decode_tree_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, int max_len, int cache_dtype) {
-    if (batch <= 0 || n <= 0 || n > kTreeMaxTokens || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || head_dim <= 0 || max_len < 0) return 0;
+    if (batch <= 0 || n <= 0 || n > kTreeMaxTokens || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || head_dim <= 0 || max_len < 0 ||
+        !fits(batch, n, n_head, n_kv_head, max_len))
+        return 0;                                          // the call refuses the same shapes
     return record_bytes(batch, n, n_head, n_kv_head, head_dim, max_len + n, cache_dtype);
 }
 
@@ -122,7 +129,8 @@ int nimllm_attn_decode_tree_paged(const void *q, int q_dtype, const void *k_page
 }
 
 size_t nimllm_attn_decode_scored_workspace_bytes(int batch, int n_head, int n_kv_head, int head_dim, int max_len, int cache_dtype) {
-    if (batch <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || head_dim <= 0 || max_len <= 0) return 0;
+    if (batch <= 0 || n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || head_dim <= 0 || max_len <= 0 || !fits(batch, 1, n_head, n_kv_head, max_len))
+        return 0;
     return record_bytes(batch, 1, n_head, n_kv_head, head_dim, max_len, cache_dtype) + round256((size_t)batch * n_head * 2 * sizeof(float)) +
            (size_t)batch * n_head * raw_rows(max_len) * sizeof(float);
 }

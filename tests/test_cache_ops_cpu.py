@@ -73,6 +73,16 @@ def test_workspaces_are_asked_for():
     assert L.nimllm_attn_decode_tree_workspace_bytes(1, 300, 4, 2, 64, 100, 1) == 0
 
 
+@pytest.mark.parametrize("shape", [dict(max_len=2**31 - 1), dict(max_len=2**30 + 1), dict(batch=65536), dict(Hq=2**30, Hkv=2**30), dict(Hq=2**31 - 2, Hkv=1)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_no_workspace_for_shapes_that_are_refused(dtype, shape):
+    a = {**dict(batch=1, n=256, Hq=4, Hkv=2, D=64, max_len=100), **shape}
+    assert L.nimllm_attn_decode_tree_workspace_bytes(*a.values(), dtype) == 0
+    refused(_tree(B=a["batch"], n=256, Hq=a["Hq"], Hkv=a["Hkv"], max_len=a["max_len"], ct=dtype), 2, "too large")
+    del a["n"]
+    assert L.nimllm_attn_decode_scored_workspace_bytes(*a.values(), dtype) == 0
+
+
 def test_paged_refusals():
     f = L.nimllm_attn_decode_tree_paged
     tail = (None, 100, None, None, P, 0, None, 1, 4, 4, 2, 64, 0.125, None, 0, None)
