@@ -315,7 +315,7 @@ int nimllm_kv_accept_paged(void *k_pages, void *v_pages, int cache_dtype, int n_
 /* nimllm_attn_decode (one token per sequence) that also keeps score of the cached rows:
  *   score[b][h][r] = decay * score[b][h][r] + sum over the query heads of KV head h of the softmax weight of row r
  * for r < seq_len[b]; score is device fp32 [batch][n_kv_head][score_rows], score_rows >= max_len; decay 0 does not
- * read the old value.  head_dim 64 or 128; workspace as above. */
+ * read the old value.  head_dim 64 or 128; at most 6144 query heads per KV head; workspace as above. */
 size_t nimllm_attn_decode_scored_workspace_bytes(int batch, int n_head, int n_kv_head, int head_dim, int max_len,
                                                  int cache_dtype);
 int nimllm_attn_decode_scored(const void *q, int q_dtype, const void *k_cache, const void *v_cache, int cache_dtype,

@@ -12,6 +12,8 @@ namespace nimllm {
 
 namespace {
 
+constexpr int kScoredMaxGroup = 6144;      // query heads of a KV head: a score block keeps 8 bytes of each in 48 KB of shared memory
+
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 size_t record_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim, int max_total, int cache_dtype) {
     return round256(cache_dtype == NIMLLM_BF16 ? tree_tc_workspace_bytes(batch, n, n_head, n_kv_head, head_dim)
@@ -80,6 +82,8 @@ int decode_scored(const char *who, const CacheRows &rows, const void *q, int q_d
     if (max_len <= 0) return fail(NIMLLM_ERR_ARG, "%s: max_len %d", who, max_len);
     if (score_rows < max_len) return fail(NIMLLM_ERR_ARG, "%s: %lld scores per KV head, max_len %d", who, (long long)score_rows, max_len);
     if (n_kv_head > 65535) return fail(NIMLLM_ERR_UNSUPPORTED, "%s: Hkv %d", who, n_kv_head);
+    if (n_head / n_kv_head > kScoredMaxGroup)
+        return fail(NIMLLM_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most %d)", who, n_head / n_kv_head, kScoredMaxGroup);
     TreeParams p = {};
     p.q = q; p.k = k; p.v = v; p.rows = rows; p.seq_len = seq_len;
     p.out = out; p.q_dtype = q_dtype; p.out_dtype = out_dtype; p.max_len = max_len; p.drafts = 0;

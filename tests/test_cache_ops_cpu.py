@@ -110,6 +110,14 @@ def test_scored_refusals():
     refused(go(), 3, "workspace")
 
 
+@pytest.mark.parametrize("heads", [6145, 8192])
+def test_scored_refuses_more_heads_than_a_block_holds(heads):
+    """The update of the scores would not launch, behind an attention that has."""
+    a = dict(q=P, qt=0, k=P, v=P, ct=1, off=None, ss=65536, hs=16384, cap=128, len=None, max_len=100, out=P, ot=0, score=P, rows=100, decay=1.0,
+             B=1, Hq=heads, Hkv=1, D=64, scale=0.125, ws=None, bytes=0, st=None)
+    refused(L.nimllm_attn_decode_scored(*a.values()), 2, "query heads per KV head")
+
+
 def test_accept_refusals():
     f = L.nimllm_kv_accept
 
