@@ -115,3 +115,25 @@ def test_scores_of_rows_that_count_as_hidden(cache_dtype, Hq):
     assert torch.isfinite(out).all() and torch.isfinite(score).all()
     added = (score - 1.5).sum(-1)                          # nothing, or the equal weights of a softmax
     assert ((added == 0) | ((added - Hq // Hkv).abs() < 1e-3)).all()
+
+
+@pytest.mark.parametrize("cache_dtype", [F, H])
+@pytest.mark.parametrize("n,Hq,Hkv", [(2, 4, 2), (24, 2, 1)])
+def test_more_sequences_than_threads(cache_dtype, n, Hq, Hkv):
+    rng = random.Random(7)
+    _tree_case(71, [0 if b % 7 == 3 else rng.randint(0, 70) for b in range(700)], n, Hq, Hkv, 64, H, cache_dtype, F, 0, "tree")
+
+
+def test_calls_repeat_themselves_bit_for_bit():
+    for types in ((F, F, F), (F, H, F), (H, H, H)):
+        for n, Hq in ((1, 8), (5, 8), (24, 8), (64, 8)):
+            cache = U.Cache(81, [5000 + n, 17 + n, 2600 + n], 2, 128, types[1], 64, cap=5100)
+            q = torch.randn(3, n, Hq * 128, device="cuda").to(types[0])
+            kw = dict(n_head=Hq, n_kv_head=2, head_dim=128, max_len=5000, out_dtype=types[2], seq_len=torch.tensor([5000, 17, 2600], dtype=torch.int32).cuda())
+            a = A.decode_tree_paged(q, cache.kd, cache.vd, cache.table, **kw)
+            sa = torch.zeros(3, 2, 5000, device="cuda")
+            oa = A.decode_scored_paged(q[:, 0].contiguous(), cache.kd, cache.vd, cache.table, sa, **kw)
+            for _ in range(5):
+                assert torch.equal(a, A.decode_tree_paged(q, cache.kd, cache.vd, cache.table, **kw))
+                s = torch.zeros_like(sa)
+                assert torch.equal(oa, A.decode_scored_paged(q[:, 0].contiguous(), cache.kd, cache.vd, cache.table, s, **kw)) and torch.equal(s, sa)

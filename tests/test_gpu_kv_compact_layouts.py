@@ -4,6 +4,7 @@ import random
 import pytest
 import torch
 
+import cache_util as U
 from nimllm_b200 import attention as A
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,26 @@ def test_layouts(dtype, layer, seq, head):
     for i, x in enumerate(at[: B * HKV]):                  # layer 0
         want[x, :12] = k1.view(-1, CAP, D)[x, kept[i // HKV, i % HKV].long()]
     assert torch.equal(kc.view(-1, CAP, D), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_accept_in_pages_of_several_layers(dtype):
+    rng = random.Random(3)
+    layers, n, Hkv, D, lens = 4, 9, 2, 64, [30, 0, 61]
+    c = U.Cache(90, [l + n for l in lens], Hkv, D, dtype, 32)
+    g = torch.Generator().manual_seed(91)
+    kp, vp = (torch.randn(layers, *c.kd.shape, generator=g).to(dtype).cuda() for _ in range(2))
+    k0, v0 = kp.clone(), vp.clone()
+    paths = [sorted(rng.sample(range(n), 5)) for _ in lens]
+    new = A.kv_accept_paged(kp, vp, c.table, torch.tensor(paths, dtype=torch.int32).cuda(), torch.tensor([5, 3, 4], dtype=torch.int32).cuda(),
+                            torch.tensor(lens, dtype=torch.int32).cuda(), n_draft=n, n_kv_head=Hkv, head_dim=D, n_layer=layers)
+    assert new.tolist() == [35, 3, 65]
+    for now, before in ((kp, k0), (vp, v0)):
+        for layer in range(layers):
+            want = before[layer].clone()
+            for b, (L, m) in enumerate(zip(lens, (5, 3, 4))):
+                for i in range(m):
+                    to, fro = L + i, L + paths[b][i]
+                    tp, fp = int(c.table_host[b, to // 32]), int(c.table_host[b, fro // 32])
+                    want[tp, :, to % 32] = before[layer][fp, :, fro % 32]
+            assert torch.equal(now[layer], want)
