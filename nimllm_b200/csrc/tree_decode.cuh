@@ -26,7 +26,7 @@ struct TreeParams {
     // workspace
     float *recs;                 // pieces of split rows: {o[D], m, l, 0, 0}
     float *raw;                  // scored: scaled scores in log2 units, [B][Hq][raw_ld]
-    float *stats;                // scored: {m in log2 units, 1 / l} per [B][Hq]
+    float *stats;                // scored: {m in log2 units, l} per [B][Hq], l = -1: the row was cut
     int64_t raw_ld;
     int chunk_rows, max_chunks;
 };
@@ -53,7 +53,7 @@ __device__ __forceinline__ int64_t tree_out_row(const TreeParams &p, int b, int 
 }
 
 // 1 / l for the sum l of a softmax, 0 for a row that attends nothing.  NaN stays NaN, and an infinite sum times the 0 that it gives.
-__device__ __forceinline__ float inverse_sum(float l) { return l != 0.f ? 1.f / l : 0.f; }
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : l; }
 
 // the kernels for bf16 caches (tree_wide_tc.cu, tree_narrow_tc.cu) and for fp32 caches (tree_f32.cu)
 size_t tree_tc_workspace_bytes(int batch, int n, int n_head, int n_kv_head, int head_dim);

@@ -76,6 +76,10 @@ template <int D> __device__ __forceinline__ void pieces_stats(const Pieces &x, i
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
 }
 
+// What the scores of a row are worked out from, exp2(raw - m) / l.  l - l: without a finite sum there is no reference either, so that they are
+// all NaN; without any weight the reference is above them all.
+__device__ __forceinline__ float2 score_stats(float m, float l) { return make_float2(l != 0.f ? m + (l - l) : INFINITY, inverse_sum(l)); }
+
 // One block joins up to 32 rows that are cut alike.  `out_row(r)` is row r's row of out.
 // First every (row, piece) statistic is fetched at once and turned into the piece's weight, then every 16 bytes of the rows is a sum
 // over the pieces whose loads wait for nothing else.
@@ -208,22 +212,30 @@ __global__ void __launch_bounds__(kFinishThreads, 4) tree_finish_kernel(TreePara
     int row = r0 + threadIdx.x * 4;
     Ahead now;
     fetch(now, row);
-    for (int g = threadIdx.x; g < p.G; g += kFinishThreads) s_stat[g] = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + g));
+    for (int g = threadIdx.x; g < p.G; g += kFinishThreads) {
+        const float2 t = *reinterpret_cast<const float2 *>(p.stats + 2 * (h0 + g));
+        s_stat[g] = t.y < 0.f ? t : score_stats(t.x, t.y);
+    }
     const int len = tree_committed(p, b);
     if (r0 >= len) return;
     __syncthreads();
-    // a negative sum marks a row that was cut: its pieces are joined here.  Every head is asked by itself: heads in different query tiles
-    // (128 or 256 of them) are cut apart from one another.  A head's entry is read and written by one warp.
-    for (int g = warp; g < p.G; g += kFinishThreads / 32) {
-        const bool cut = s_stat[g].y < 0.f;
-        __syncwarp();
-        if (!cut) continue;
-        const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g, len, p.G) : chunk_pieces<D>(p, h0 + g, len);
-        float M, L;
-        pieces_stats<D>(pc, lane, M, L);
-        if (lane == 0) s_stat[g] = score_stats(M * kLog2e, L);
+    // A negative sum marks a row that was cut: its pieces are joined here.  Every head is asked by itself: heads in different query tiles
+    // (128 or 256 of them) are cut apart from one another.  A head's entry is read and written by one warp, once all warps have looked.
+    bool cut = false;
+    for (int g = lane; g < p.G; g += 32) cut |= s_stat[g].y < 0.f;
+    if (__any_sync(0xffffffffu, cut)) {
+        __syncthreads();
+        for (int g = warp; g < p.G; g += kFinishThreads / 32) {
+            const bool cut_g = s_stat[g].y < 0.f;
+            __syncwarp();
+            if (!cut_g) continue;
+            const Pieces pc = f.workers ? tc_pieces<D>(p, f, b, kvh, g, len, p.G) : chunk_pieces<D>(p, h0 + g, len);
+            float M, L;
+            pieces_stats<D>(pc, lane, M, L);
+            if (lane == 0) s_stat[g] = score_stats(M * kLog2e, L);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     for (; row < min(len, r0 + kScoreRows); row += 4 * kFinishThreads) {
         Ahead next;
         if (row + 4 * kFinishThreads < min(len, r0 + kScoreRows)) fetch(next, row + 4 * kFinishThreads);

@@ -165,13 +165,10 @@ __device__ __forceinline__ void store_row8(const TreeParams &p, int64_t orow, in
         store_row4<D>(p, orow, d + 4, make_float4(x[4], x[5], x[6], x[7]));
     }
 }
-// What the scores of a row are worked out from, exp2(raw - m) / l.  l - l: without a finite sum there is no reference either, so that they are
-// all NaN; without any weight the reference is above them all.
-__device__ __forceinline__ float2 score_stats(float m, float l) { return make_float2(l != 0.f ? m + (l - l) : INFINITY, inverse_sum(l)); }
 template <int D>
 __device__ __forceinline__ void store_row_stats(const TreeParams &p, int64_t orow, float m, float l) {
     if (p.partials_out) *reinterpret_cast<float4 *>(p.partials_out + orow * (D + 4) + D) = make_float4(m * kLn2, l, 0.f, 0.f);
-    if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = score_stats(m, l);
+    if (p.stats) *reinterpret_cast<float2 *>(p.stats + 2 * orow) = make_float2(m, l);
 }
 
 // a row that was cut has no statistics yet: the score blocks join its pieces themselves
