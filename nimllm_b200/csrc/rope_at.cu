@@ -10,7 +10,7 @@
 // bf16, 4 for fp32; else 4), all of them rotated or all of them passed.
 //
 // Measured (graph replay): gradient of 4 x 8192 tokens, 32 + 8 heads of 128, bf16: 127 us = 5.3 TB/s; 61 trees of 24 tokens into pages:
-// 10.3 us (5.6 us of memory time, the rest is launch and two dependent loads, pos and then tables); one token 4.1 us.
+// 10.3 us (5.6 us of memory time, the rest is launch and three loads in a row, pos, tables and the page entry); one token 4.1 us.
 #include <math.h>
 
 #include "cache_rows.cuh"

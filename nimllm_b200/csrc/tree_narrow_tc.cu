@@ -7,9 +7,11 @@
 // same MMA, so that 32-bit precision costs little tensor time.  An fp32 q and the P of fp32 results have three terms (2^-26 left), the P
 // of bf16 results two (2^-17 left).
 //
-// HBM-bound.  Measured (graph replay): 256 sequences of 512 - 4096 rows, 5 tokens, 9 q / 3 kv heads of 64, fp32 q and results: 118 us,
-// of which the rows' bytes are 70 (3.9 TB/s: segments of a few tiles each, every one with its own Q, first maximum and join); scored
-// decode of 32 sequences of 2 - 8 K rows in pages, 32 q / 8 kv heads of 128, bf16: 138 us, 104 at the measured peak (4.9 TB/s).
+// Measured (graph replay): scored decode of 32 sequences of 2 - 8 K rows in pages, 32 q / 8 kv heads of 128, bf16: 122 us, 104 at the
+// measured peak of HBM (5.6 TB/s).  256 sequences of 512 - 4096 rows, 5 tokens, 9 q / 3 kv heads of 64, fp32 q and results: 118 us, of which
+// the rows' bytes are 70: tiles of head size 64 have half the bytes and are bound by what a tile costs, whatever its segment.  A CTA has
+// about 94 tiles in five segments, 1.15 us or 2200 cycles each (64 sequences with segments of 24 tiles: 1.19 us): a softmax group
+// writes its next P only behind its own P V, and 128 threads vote once a tile.  The tensor pipe is active for 12 % of that launch, DRAM 43 %.
 //
 //   warps 0-3, 4-7   two softmax groups, taking the tiles of 128 rows in turn: the waits of one hide behind the other
 //   warps 8-11       K rows (8, 9) and V rows (10, 11) into a ring of slots with cp.async, swizzled, exact to the row
@@ -623,7 +625,8 @@ template <int D> cudaError_t launch_narrow_d(const TreeParams &p, TcArgs &a, cud
 
 }  // namespace
 
-// P's terms are columns of one 64-column operand; 96 columns of Q at head size 128 would leave two slots.
+// P's terms are columns of one 64-column operand; 96 columns of Q at head size 128 would leave two slots.  So the rule is the operand's width,
+// not a crossing of two times: fp32 results go from 84 us at 16 rows to 195 at 24, where the wide kernel has to take them.
 // 32 sequences of 2 - 4 K rows, 32 q / 8 kv heads of 128, here and in tree_wide_tc.cu: bf16, 8 rows 76 and 96 us, 16 rows 79 and 95,
 // 24 rows 91 and 97, 32 rows 96 and 99; fp32 q and results, 8 rows 76 and 193, 16 rows 84 and 192.  64 sequences, 9 q / 3 kv heads of 64,
 // fp32 q and bf16 results: 15 rows 47 and 72, 30 rows 69 and 74.

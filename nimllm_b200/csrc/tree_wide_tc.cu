@@ -26,10 +26,11 @@
 // well, so that l is the sum of the weights themselves, which the scores are divided by (32 sequences of 2 - 4 K rows, 40 heads of 128:
 // 102 us, with one term 100).
 //
-// Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 152 us (160 without the
-// rows' policy of leaving L2 first, which keeps records, Q and code there).  The rows' bytes at the measured peak of HBM are 65 us, the
-// products at the library's matrix rate 64.  A tile takes 2700 cycles: its 24 products 2200 - the tensor core takes about 93 cycles for
-// one, 64 columns wide or 128 - and its exponentials 1024 of the two groups' turns.  Tiles of 128 rows, which need 16 products for the
+// Measured (graph replay): 8 trees of 64 tokens over 9 - 16 K rows in pages, 32 q / 8 kv heads of 128, bf16: 148 us (172 call by call from
+// Python; 8 us more without the rows' policy of leaving L2 first, which keeps records, Q and code there).  The rows' bytes at the measured
+// peak of HBM are 65 us, the products at the library's matrix rate 64.  A tile takes 2700 cycles, 2200 of them from its first product to its
+// last: 24 products that follow one another every 93 cycles or so, 64 columns wide or 128, while the tensor pipe is active for 36 % of the
+// cycles.  Its exponentials take 1024 of the two groups' turns.  Tiles of 128 rows, which need 16 products for the
 // same work, were built with one S of both groups and with P over S, before that policy: 179 and 199 us for 168, because a group then
 // waits for the other's reading of S or for its own P.
 //
