@@ -277,9 +277,9 @@ int nimllm_rope_at_bwd(const void *dq_rot, void *dq, int n_head, const void *dk_
  *              ancestors and itself); NULL: a chain, drafts 0 .. i.  A token without any row to attend gets zeros
  *   partials_out  optional fp32 [batch*n*n_head, head_dim + 4] records as in nimllm_attn_decode (out may be NULL then)
  *   head_dim   64 or 128.  The arithmetic is that of 32 bits for either cache type, but for bf16 results of more than 32
- *              query rows (n * n_head / n_kv_head), whose softmax weights are rounded to bf16 (fp32 results
- *              have them in 32 bits for any number).  Every row of V up to the last draft must be finite even where a mask hides it (a hidden row of K may hold anything); a row whose
- *              scaled score is below -5e29 may count as hidden
+ *              query rows (n * n_head / n_kv_head), whose softmax weights are rounded to bf16 (fp32 results have them in
+ *              32 bits for any number).  Every row of V up to the last draft must be finite even where a mask hides it (a
+ *              hidden row of K may hold anything); a row whose scaled score is below -5e29 may count as hidden
  *   workspace  256-byte aligned, nimllm_attn_decode_tree_workspace_bytes(...) bytes
  * The kernel for bf16 caches (also that of nimllm_attn_decode_scored) bounds its internal waits, about 2 s without
  * progress; nimllm_attn_decode_tree_status tells as nimllm_attn_prefill_status does whether one gave up. */
